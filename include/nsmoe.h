@@ -47,7 +47,9 @@ int32_t nsmoe_abi_version(void);
  * the library records a HIP event pair on the launch stream around each launch of its
  * main kernels ("pack", "route_fwd", "dispatch", "expert_fwd", "combine",
  * "expert_bwd", "expert_dx", "dw" (or "dw_in" and "dw_out" where they run apart),
- * "combine_dx", "router_dw", "route_bwd", "norm_bwd", "attn_k_prep", "attn_fwd", "ce_rows", "norm_fwd") until
+ * "combine_dx", "router_dw", "route_bwd", "norm_bwd", "attn_k_prep", "attn_fwd", "ce_rows", "norm_fwd", "rope",
+ * "logits", "evict_select", "evict_move",
+ * "prefix_part", "own_part", "prefix_join") until
  * `capacity` pairs are used.
  * nsmoe_timing_read waits for the recorded events of one kernel and returns their
  * summed duration.  capacity 0 disables timing and frees the events. */
@@ -444,6 +446,174 @@ int nsmoe_linear(int32_t dtype, const void* x, int64_t n_rows, int32_t k, int32_
 int nsmoe_cross_entropy_rows(int32_t dtype, const void* logits, int64_t ld, int64_t n_rows,
                              int32_t vocab, const int64_t* target, int64_t ignore_index,
                              const int64_t* n_valid, float* loss, void* grad, void* stream);
+
+/* ---- rotary positions ------------------------------------------------------------------
+ * The rotation of src/model/rope.py as an operator of its own, for any positions:
+ *   y1 = amplitude (x1 cos t - x2 sin t), y2 = amplitude (x2 cos t + x1 sin t),
+ *   t = positions[b, i] * freqs[j] (radians, fp64), j < rot_dim / 2
+ * over the dims (j, j + rot_dim / 2) of a head, or (2 j, 2 j + 1) when `interleaved`; dims
+ * from rot_dim on are copied.  `inverse` turns the other way (the gradient of the rotation).
+ * q [batch, n_tokens, n_q, head_dim] and k [batch, n_tokens, n_k, head_dim] in one launch
+ * (n_q or n_k may be 0); strides in elements over (batch, token, head), the last dim
+ * contiguous.  q_out / k_out may be q / k themselves with the same strides (in place), and
+ * must not overlap them otherwise.  bf16, fp16, fp32; fp32 arithmetic, rounded once.
+ * rot_dim even, at most head_dim, head_dim at most 1024. */
+typedef struct nsmoe_rope_args {
+  int32_t dtype;
+  int32_t interleaved;
+  int32_t inverse;
+  float amplitude;
+  int64_t batch;
+  int64_t n_tokens;
+  int32_t n_q;
+  int32_t n_k;
+  int32_t head_dim;
+  int32_t rot_dim;
+  const void* q;
+  const void* k;
+  void* q_out;
+  void* k_out;
+  int64_t q_stride[3];
+  int64_t k_stride[3];
+  int64_t q_out_stride[3];
+  int64_t k_out_stride[3];
+  const int64_t* positions; /* strides pos_stride over (batch, token), 0 to broadcast */
+  int64_t pos_stride[2];
+  const double* freqs; /* [rot_dim / 2] */
+} nsmoe_rope_args;
+
+int nsmoe_rope(const nsmoe_rope_args* args, void* stream);
+
+/* ---- penalties, bias and grammar mask on logits -----------------------------------------
+ * Between the head's logits and the choice of a token (no counterpart in the reference).  For
+ * row b and token v, with h = history[b, 0 .. lens[b]) (int64; ids outside [0, vocab) count
+ * nothing), prompt_lens[b] of it the prompt:
+ *   x = logits[b, v];  x = x > 0 ? x / repetition[b] : x * repetition[b]  if v is in h
+ *   x -= frequency[b] n + presence[b] [n > 0],  n = times v occurs in h after the prompt
+ *   x += bias[b, v];   x = -inf where bit v % 32 of mask[b, v / 32] is 0
+ * in fp32, rounded once.  lens, prompt_lens (int32), repetition, frequency, presence (fp32,
+ * [batch]), bias (fp32) and mask (int32 words) may each be NULL: no such term, every row's
+ * whole history, no prompt.  Row strides in elements (words for the mask), 0 to broadcast a
+ * bias or mask row.  out may be logits itself (the same type and stride); out_dtype is dtype
+ * or fp32.  batch at most 65535; a mask row has ceil(vocab / 32) words. */
+typedef struct nsmoe_logits_args {
+  int32_t dtype;
+  int32_t out_dtype;
+  int64_t batch;
+  int32_t vocab;
+  int32_t reserved;
+  const void* logits;
+  void* out;
+  int64_t logits_stride;
+  int64_t out_stride;
+  const int64_t* history;
+  int64_t history_stride;
+  int64_t history_cap; /* columns of history */
+  const int32_t* lens;
+  const int32_t* prompt_lens;
+  const float* repetition;
+  const float* frequency;
+  const float* presence;
+  const float* bias;
+  int64_t bias_stride;
+  const int32_t* mask;
+  int64_t mask_stride;
+} nsmoe_logits_args;
+
+int nsmoe_penalize_logits(const nsmoe_logits_args* args, void* stream);
+
+/* ---- eviction from a key/value cache ----------------------------------------------------
+ * Keeps, of each (sequence, key/value head) of a cache, the rows that attention has weighted
+ * most (no counterpart in the reference).  With n = lens[b]: n <= budget keeps all; otherwise
+ * the first `sinks` rows, the last `recent` and the budget - sinks - recent others with the
+ * largest weights[b, h, .] (ties: the lower index; NaN counts as the largest).  Kept rows go
+ * to the front of the outputs in index order.
+ *   k, v [batch, cap, n_kv_heads, head_dim], elements of elem_bytes (2 or 4), strides in
+ *     elements over (batch, row, head), the last dim contiguous; weights [batch, n_kv_heads,
+ *     cap] fp32, strides over (batch, head); lens [batch] int32.
+ *   k_out, v_out, weights_out likewise with out_cap >= budget rows, sharing no memory with the
+ *     inputs.  Rows from the new length on are left as they were, or zeroed with zero_tail.
+ *   index [batch, n_kv_heads, budget] int32: the old index of each kept row, -1 behind them;
+ *   lens_out [batch] int32 = min(n, budget) (not lens itself). */
+typedef struct nsmoe_evict_args {
+  int32_t elem_bytes;
+  int32_t n_kv_heads;
+  int32_t head_dim;
+  int32_t zero_tail;
+  int64_t batch;
+  int64_t cap;
+  int64_t out_cap;
+  int64_t budget;
+  int64_t recent;
+  int64_t sinks;
+  const void* k;
+  const void* v;
+  void* k_out;
+  void* v_out;
+  int64_t k_stride[3];
+  int64_t v_stride[3];
+  int64_t k_out_stride[3];
+  int64_t v_out_stride[3];
+  const float* weights;
+  float* weights_out;
+  int64_t weights_stride[2];
+  int64_t weights_out_stride[2];
+  const int32_t* lens;
+  int32_t* lens_out;
+  int32_t* index;
+} nsmoe_evict_args;
+
+int nsmoe_cache_evict(const nsmoe_evict_args* args, void* stream);
+
+/* ---- attention over a shared prefix and a cache ------------------------------------------
+ * The grouped-query attention of src/model/mha.py:245-287 for a batch whose sequences share a
+ * prefix and have a cache of their own behind it (the reference decodes with one cache per
+ * sequence).  Query i < n_new of sequence b stands at row lens[b] - n_new + i of its cache: it
+ * sees the prefix's rows and its own up to that one, the last `window` of them (itself
+ * counted; 0: all).  A query whose row would be negative (lens[b] < n_new) sees nothing: its
+ * output is 0 and its lse -inf.  Keys are taken as they lie there (normalised, rotated).
+ *   q [batch, n_new, n_heads, head_dim], strides over (batch, token, head)
+ *   k_prefix, v_prefix [prefix_len, n_kv_heads, head_dim], strides over (row, head)
+ *   k, v [batch, cap, n_kv_heads, head_dim], strides over (batch, row, head); rows from
+ *     lens[b] (int32, clamped to 0 .. cap) on are never read
+ *   out [batch, n_new, n_heads, head_dim] contiguous; lse [batch, n_new, n_heads] fp32 or NULL
+ *   weights_out [batch, n_kv_heads, cap] fp32 or NULL: weights (the same shape; NULL is zero;
+ *     may be weights_out) plus each cached row's softmax weight summed over the new queries
+ *     and the heads of its group; n_new * n_heads / n_kv_heads at most 64 with it.
+ * 16-bit types, head_dim 64 or 128, scale > 0; pointers and strides multiples of 16 bytes, the
+ * last dim contiguous.  Query head h reads key/value head h / (n_heads / n_kv_heads).
+ * workspace: 16-byte aligned, nsmoe_prefix_attention_workspace_size(args) bytes. */
+typedef struct nsmoe_prefix_attn_args {
+  int32_t dtype;
+  int32_t head_dim;
+  int32_t n_heads;
+  int32_t n_kv_heads;
+  int64_t batch;
+  int64_t n_new;
+  int64_t prefix_len;
+  int64_t cap;
+  int32_t window;
+  float scale;
+  const void* q;
+  const void* k_prefix;
+  const void* v_prefix;
+  const void* k;
+  const void* v;
+  int64_t q_stride[3];
+  int64_t kp_stride[2];
+  int64_t vp_stride[2];
+  int64_t k_stride[3];
+  int64_t v_stride[3];
+  const int32_t* lens;
+  void* out;
+  float* lse;
+  const float* weights;
+  float* weights_out;
+} nsmoe_prefix_attn_args;
+
+size_t nsmoe_prefix_attention_workspace_size(const nsmoe_prefix_attn_args* args);
+int nsmoe_prefix_attention(const nsmoe_prefix_attn_args* args, void* workspace,
+                           size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

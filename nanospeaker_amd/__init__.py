@@ -5,12 +5,16 @@ C ABI (include/nsmoe.h) and the reference's Python interface (MoEBlock, TopKRout
 moe_kernel ops).
 """
 
+from .cache import cache_evict, shared_prefix_attention
 from .glu import GLUFeedForward, glu_hidden_dim, make_glu
+from .logits import penalize_logits
 from .moe import AUTO_CAPACITY, MoEBlock
+from .rope import rotary_embed, rotary_frequencies
 from .router import TopKRouter
 from .utils import ACTIVATIONS, resolve_activation
 
 __all__ = [
-    "ACTIVATIONS", "AUTO_CAPACITY", "GLUFeedForward", "MoEBlock", "TopKRouter",
-    "glu_hidden_dim", "make_glu", "resolve_activation",
+    "ACTIVATIONS", "AUTO_CAPACITY", "GLUFeedForward", "MoEBlock", "TopKRouter", "cache_evict",
+    "glu_hidden_dim", "make_glu", "penalize_logits", "resolve_activation", "rotary_embed",
+    "rotary_frequencies", "shared_prefix_attention",
 ]

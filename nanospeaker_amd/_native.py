@@ -55,6 +55,61 @@ class AttnArgs(ctypes.Structure):
     ]
 
 
+class RopeArgs(ctypes.Structure):
+    """Mirror of `nsmoe_rope_args`."""
+
+    _fields_ = [
+        ("dtype", _i32), ("interleaved", _i32), ("inverse", _i32), ("amplitude", ctypes.c_float),
+        ("batch", _i64), ("n_tokens", _i64),
+        ("n_q", _i32), ("n_k", _i32), ("head_dim", _i32), ("rot_dim", _i32),
+        ("q", _vp), ("k", _vp), ("q_out", _vp), ("k_out", _vp),
+        ("q_stride", _i64 * 3), ("k_stride", _i64 * 3), ("q_out_stride", _i64 * 3),
+        ("k_out_stride", _i64 * 3),
+        ("positions", _vp), ("pos_stride", _i64 * 2), ("freqs", _vp),
+    ]
+
+
+class LogitsArgs(ctypes.Structure):
+    """Mirror of `nsmoe_logits_args`."""
+
+    _fields_ = [
+        ("dtype", _i32), ("out_dtype", _i32), ("batch", _i64), ("vocab", _i32),
+        ("reserved", _i32), ("logits", _vp), ("out", _vp), ("logits_stride", _i64),
+        ("out_stride", _i64), ("history", _vp), ("history_stride", _i64),
+        ("history_cap", _i64), ("lens", _vp), ("prompt_lens", _vp), ("repetition", _vp),
+        ("frequency", _vp), ("presence", _vp), ("bias", _vp), ("bias_stride", _i64),
+        ("mask", _vp), ("mask_stride", _i64),
+    ]
+
+
+class EvictArgs(ctypes.Structure):
+    """Mirror of `nsmoe_evict_args`."""
+
+    _fields_ = [
+        ("elem_bytes", _i32), ("n_kv_heads", _i32), ("head_dim", _i32), ("zero_tail", _i32),
+        ("batch", _i64), ("cap", _i64), ("out_cap", _i64), ("budget", _i64), ("recent", _i64),
+        ("sinks", _i64), ("k", _vp), ("v", _vp), ("k_out", _vp), ("v_out", _vp),
+        ("k_stride", _i64 * 3), ("v_stride", _i64 * 3), ("k_out_stride", _i64 * 3),
+        ("v_out_stride", _i64 * 3), ("weights", _vp), ("weights_out", _vp),
+        ("weights_stride", _i64 * 2), ("weights_out_stride", _i64 * 2),
+        ("lens", _vp), ("lens_out", _vp), ("index", _vp),
+    ]
+
+
+class PrefixAttnArgs(ctypes.Structure):
+    """Mirror of `nsmoe_prefix_attn_args`."""
+
+    _fields_ = [
+        ("dtype", _i32), ("head_dim", _i32), ("n_heads", _i32), ("n_kv_heads", _i32),
+        ("batch", _i64), ("n_new", _i64), ("prefix_len", _i64), ("cap", _i64),
+        ("window", _i32), ("scale", ctypes.c_float),
+        ("q", _vp), ("k_prefix", _vp), ("v_prefix", _vp), ("k", _vp), ("v", _vp),
+        ("q_stride", _i64 * 3), ("kp_stride", _i64 * 2), ("vp_stride", _i64 * 2),
+        ("k_stride", _i64 * 3), ("v_stride", _i64 * 3),
+        ("lens", _vp), ("out", _vp), ("lse", _vp), ("weights", _vp), ("weights_out", _vp),
+    ]
+
+
 class BlockNorm(ctypes.Structure):
     """Mirror of `nsmoe_block_norm`."""
 
@@ -106,6 +161,11 @@ SIGNATURES = {
                                       _vp]),
     "nsmoe_attn_prefill": (ctypes.c_int, [ctypes.POINTER(AttnArgs), _vp]),
     "nsmoe_linear": (ctypes.c_int, [_i32, _vp, _i64, _i32, _i32, _vp, _vp, _vp, _vp]),
+    "nsmoe_rope": (ctypes.c_int, [ctypes.POINTER(RopeArgs), _vp]),
+    "nsmoe_penalize_logits": (ctypes.c_int, [ctypes.POINTER(LogitsArgs), _vp]),
+    "nsmoe_cache_evict": (ctypes.c_int, [ctypes.POINTER(EvictArgs), _vp]),
+    "nsmoe_prefix_attention_workspace_size": (_sz, [ctypes.POINTER(PrefixAttnArgs)]),
+    "nsmoe_prefix_attention": (ctypes.c_int, [ctypes.POINTER(PrefixAttnArgs), _vp, _sz, _vp]),
     "nsmoe_cross_entropy_rows": (ctypes.c_int, [_i32, _vp, _i64, _i64, _i32, _vp, _i64, _vp,
                                                 _vp, _vp, _vp]),
 }

@@ -1,0 +1,272 @@
+// Eviction from a key/value cache by accumulated attention weight.
+//
+// For a sequence b with n = lens[b] cached rows and a budget of m: where n <= m every row is
+// kept; otherwise the first `sinks` rows, the last `recent` and, of those between, the
+// r = m - sinks - recent with the largest weights w[b, h, .] (ties: the lower index), chosen
+// for each key/value head h on its own.  Kept rows move to the front in index order.
+//
+//   evict_select_kernel  one workgroup per (sequence, head): the r-th largest weight by a
+//                        radix descent over order-preserving 32-bit keys (histograms of 11, 11
+//                        and 10 bits in LDS), then one ordered pass that writes the kept
+//                        indices, weights and the new length.  Each wave owns a contiguous
+//                        run of the row, so an index's place is the counts of the waves
+//                        before it plus a ballot within the wave.
+//   evict_move_kernel    copies the kept key and value rows, 16 bytes a thread, by those
+//                        indices.
+//
+// The selection reads a row of weights four times, from L2 after the first; the move reads and
+// writes the kept rows once, which is nearly all of the traffic: bound by HBM at large caches,
+// by the selection's chain of passes at small ones.
+//
+// Weights order as floats with -0 equal to +0; a NaN counts as the largest (it is kept, where
+// it can be seen, rather than lost).
+#include "../../include/nsmoe.h"
+#include "gemm_core.h"
+#include "nsmoe_capi_internal.h"
+
+namespace nsmoe {
+
+constexpr int EV_NT = 1024;
+constexpr int EV_WAVES = EV_NT / 64;
+constexpr int EV_BINS = 2048;
+constexpr int EV_MOVE_NT = 256;
+
+struct EvictParams {
+  const char *k, *v;
+  char *k_out, *v_out;
+  int64_t ksb, kst, ksh, vsb, vst, vsh;        // bytes: batch, row, head
+  int64_t kob, kot, koh, vob, vot, voh;
+  const float* w;
+  float* w_out;
+  int64_t wsb, wsh, wob, woh;                  // elements: batch, head
+  const int32_t* lens;
+  int32_t* lens_out;
+  int32_t* index;                              // [B, H, m]
+  int64_t S, So;                               // rows of the cache and of the output
+  int B, H, m, recent, sinks, row_bytes, zero_tail;
+};
+
+// Keys whose unsigned order is the weights' order: NaN above everything, -0 as +0.
+__device__ __forceinline__ uint32_t evict_key(float f) {
+  if (f != f) return 0xffffffffu;
+  const uint32_t u = __float_as_uint(f + 0.0f);  // -0 + 0 = +0
+  return (u >> 31) ? ~u : u | 0x80000000u;
+}
+
+__device__ __forceinline__ int evict_len(const EvictParams& p, int b) {
+  const int64_t n = p.lens[b];
+  return (int)(n < 0 ? 0 : n > p.S ? p.S : n);
+}
+
+__global__ void __launch_bounds__(EV_NT) evict_select_kernel(EvictParams p) {
+  __shared__ uint32_t s_hist[EV_BINS];
+  __shared__ uint32_t s_wave[EV_WAVES], s_wave2[EV_WAVES];
+  __shared__ uint32_t s_bin, s_left;
+  const int b = blockIdx.x / p.H, h = blockIdx.x % p.H;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int n = evict_len(p, b), m = p.m;
+  const float* w = p.w + b * p.wsb + h * p.wsh;
+  float* wo = p.w_out + b * p.wob + h * p.woh;
+  int32_t* idx = p.index + (int64_t)blockIdx.x * m;
+  const int kept = n < m ? n : m;
+  if (h == 0 && tid == 0) p.lens_out[b] = kept;
+  // Behind the kept rows: no index, and the weights of a buffer of our own are zero.
+  for (int i = kept + tid; i < m; i += EV_NT) idx[i] = -1;
+  if (p.zero_tail)
+    for (int64_t i = kept + tid; i < p.So; i += EV_NT) wo[i] = 0.0f;
+  if (n <= m) {
+    for (int i = tid; i < n; i += EV_NT) {
+      idx[i] = i;
+      wo[i] = w[i];
+    }
+    return;
+  }
+  const int lo = p.sinks, hi = n - p.recent;  // the rows that compete
+  uint32_t left = (uint32_t)(m - p.sinks - p.recent);
+  // The descent: `prefix` holds the decided high bits of the threshold key, `left` how many
+  // keys are still to be taken among those that share it.  left == 0 takes none: any
+  // threshold above every key would do, and the top one with no ties taken is such.
+  uint32_t prefix = 0, mask = 0;
+  const int shift[3] = {21, 10, 0}, bits[3] = {11, 11, 10};
+  for (int pass = 0; pass < 3; ++pass) {
+    const int sh = shift[pass], nb = 1 << bits[pass];
+    for (int i = tid; i < nb; i += EV_NT) s_hist[i] = 0;
+    __syncthreads();
+    for (int i = lo + tid; i < hi; i += EV_NT) {
+      const uint32_t key = evict_key(w[i]);
+      if ((key & mask) == prefix) atomicAdd(&s_hist[(key >> sh) & (nb - 1)], 1u);
+    }
+    __syncthreads();
+    // The bin, from the top, in which the running count reaches `left`: thread t holds two
+    // bins (the second histogram half is empty for 10 bits).
+    const int b1 = nb - 1 - 2 * tid, b0 = b1 - 1;
+    const uint32_t c1 = b1 >= 0 ? s_hist[b1] : 0, c0 = b0 >= 0 ? s_hist[b0] : 0;
+    const uint32_t incl = (uint32_t)wave_scan_incl((int)(c1 + c0));
+    if (lane == 63) s_wave[wave] = incl;
+    __syncthreads();
+    uint32_t before = incl - c1 - c0;
+    for (int k = 0; k < wave; ++k) before += s_wave[k];
+    // exactly one thread holds the bin that `left` falls into (left >= 1)
+    if (left > before && left <= before + c1) {
+      s_bin = (uint32_t)b1;
+      s_left = left - before;
+    } else if (left > before + c1 && left <= before + c1 + c0) {
+      s_bin = (uint32_t)b0;
+      s_left = left - before - c1;
+    }
+    __syncthreads();
+    if (left) {
+      left = s_left;
+      prefix |= s_bin << sh;
+    } else {
+      prefix |= (uint32_t)(nb - 1) << sh;
+    }
+    mask |= (uint32_t)(nb - 1) << sh;
+    __syncthreads();
+  }
+  // Keys above `prefix` are kept, of those equal to it the first `left`.  With nothing to
+  // take, prefix is 0xffffffff: no key is above it, and left is 0.
+
+  // Each wave counts, then writes, its own run of [0, n), a multiple of 64 long.
+  const int run = ((n + EV_WAVES - 1) / EV_WAVES + 63) / 64 * 64;
+  const int w0 = wave * run, w1 = w0 + run < n ? w0 + run : n;
+  uint32_t above = 0, equal = 0;  // this lane's
+  for (int i = w0 + lane; i < w1; i += 64) {
+    const bool held = i < lo || i >= hi;
+    const uint32_t key = held ? 0 : evict_key(w[i]);
+    above += held || key > prefix;
+    equal += !held && key == prefix;
+  }
+  for (int o = 32; o; o >>= 1) above += __shfl_xor(above, o), equal += __shfl_xor(equal, o);
+  if (lane == 0) s_wave[wave] = above, s_wave2[wave] = equal;
+  __syncthreads();
+  uint32_t at = 0, ties = 0;  // kept, and ties met, before this wave's run
+  for (int k = 0; k < wave; ++k) at += s_wave[k], ties += s_wave2[k];
+  at += ties < left ? ties : left;
+  for (int i0 = w0; i0 < w1; i0 += 64) {
+    const int i = i0 + lane;
+    const bool live = i < w1;
+    const bool held = live && (i < lo || i >= hi);
+    const float f = live ? w[i] : 0.0f;
+    const uint32_t key = evict_key(f);
+    const bool tie = live && !held && key == prefix;
+    const uint64_t tb = __ballot(tie), below = ((uint64_t)1 << lane) - 1;
+    const bool take = held || (live && !held && key > prefix) ||
+                      (tie && ties + (uint32_t)__popcll(tb & below) < left);
+    const uint64_t kb = __ballot(take);
+    if (take) {
+      const uint32_t o = at + (uint32_t)__popcll(kb & below);
+      idx[o] = i;
+      wo[o] = f;
+    }
+    at += (uint32_t)__popcll(kb);
+    ties += (uint32_t)__popcll(tb);
+  }
+}
+
+// One thread per 16 bytes (VEC) or 2 bytes of a row: rows of the output in order, so a wave
+// writes neighbouring addresses.
+template <class T>
+__global__ void __launch_bounds__(EV_MOVE_NT) evict_move_kernel(EvictParams p, int64_t items,
+                                                                int rows) {
+  const int per_row = p.row_bytes / (int)sizeof(T);
+  for (int64_t it = (int64_t)blockIdx.x * EV_MOVE_NT + threadIdx.x; it < items;
+       it += (int64_t)gridDim.x * EV_MOVE_NT) {
+    const int c = (int)(it % per_row);
+    const int64_t r = it / per_row;
+    const int h = (int)(r % p.H);
+    const int64_t r2 = r / p.H;
+    const int o = (int)(r2 % rows), b = (int)(r2 / rows);
+    const int64_t at = c * (int64_t)sizeof(T);
+    const int src = o < p.m ? p.index[((int64_t)b * p.H + h) * p.m + o] : -1;
+    T kv{}, vv{};
+    if (src >= 0) {
+      kv = *(const T*)(p.k + b * p.ksb + src * p.kst + h * p.ksh + at);
+      vv = *(const T*)(p.v + b * p.vsb + src * p.vst + h * p.vsh + at);
+    } else if (!p.zero_tail) {
+      continue;
+    }
+    *(T*)(p.k_out + b * p.kob + o * p.kot + h * p.koh + at) = kv;
+    *(T*)(p.v_out + b * p.vob + o * p.vot + h * p.voh + at) = vv;
+  }
+}
+
+}  // namespace nsmoe
+
+using namespace nsmoe;
+
+extern "C" int nsmoe_cache_evict(const nsmoe_evict_args* a, void* stream) {
+  NSMOE_REQUIRE(a, "cache_evict: NULL args");
+  NSMOE_REQUIRE(a->elem_bytes == 2 || a->elem_bytes == 4, "cache_evict: elements of %d bytes",
+                a->elem_bytes);
+  NSMOE_REQUIRE(a->batch >= 0 && a->n_kv_heads >= 1 && a->head_dim >= 1 && a->head_dim <= 4096 &&
+                    a->n_kv_heads <= 4096 && a->batch * a->n_kv_heads < (1 << 24),
+                "cache_evict: bad batch, heads or head_dim");
+  NSMOE_REQUIRE(a->cap >= 0 && a->cap < (1 << 30) && a->out_cap >= 0 && a->out_cap < (1 << 30),
+                "cache_evict: bad capacity");
+  NSMOE_REQUIRE(a->budget >= 1 && a->budget <= a->out_cap,
+                "cache_evict: budget %lld outside 1 .. the output's %lld rows",
+                (long long)a->budget, (long long)a->out_cap);
+  NSMOE_REQUIRE(a->recent >= 0 && a->sinks >= 0 && a->recent + a->sinks <= a->budget,
+                "cache_evict: sinks %lld + recent %lld exceed the budget %lld",
+                (long long)a->sinks, (long long)a->recent, (long long)a->budget);
+  if (a->batch == 0) return NSMOE_OK;
+  NSMOE_REQUIRE(a->lens && a->index && a->lens_out && a->weights_out && a->k_out && a->v_out &&
+                    (a->cap == 0 || (a->k && a->v && a->weights)),
+                "cache_evict: NULL pointer");
+  NSMOE_REQUIRE(((uintptr_t)a->weights & 3) == 0 && ((uintptr_t)a->weights_out & 3) == 0,
+                "cache_evict: misaligned weights");
+  const int64_t es = a->elem_bytes;
+  EvictParams P{};
+  uint64_t bits = (uint64_t)a->k | (uint64_t)a->v | (uint64_t)a->k_out | (uint64_t)a->v_out |
+                  (uint64_t)(a->head_dim * es);
+  auto stride = [&](const int64_t* st, int64_t& sb, int64_t& sr, int64_t& sh) {
+    sb = st[0] * es, sr = st[1] * es, sh = st[2] * es;
+    bits |= (uint64_t)sb | (uint64_t)sr | (uint64_t)sh;
+  };
+  stride(a->k_stride, P.ksb, P.kst, P.ksh);
+  stride(a->v_stride, P.vsb, P.vst, P.vsh);
+  stride(a->k_out_stride, P.kob, P.kot, P.koh);
+  stride(a->v_out_stride, P.vob, P.vot, P.voh);
+  NSMOE_REQUIRE((bits & (es - 1)) == 0, "cache_evict: misaligned pointer");
+  P.k = (const char*)a->k;
+  P.v = (const char*)a->v;
+  P.k_out = (char*)a->k_out;
+  P.v_out = (char*)a->v_out;
+  P.w = a->weights;
+  P.w_out = a->weights_out;
+  P.wsb = a->weights_stride[0];
+  P.wsh = a->weights_stride[1];
+  P.wob = a->weights_out_stride[0];
+  P.woh = a->weights_out_stride[1];
+  P.lens = a->lens;
+  P.lens_out = a->lens_out;
+  P.index = a->index;
+  P.S = a->cap;
+  P.So = a->out_cap;
+  P.B = (int)a->batch;
+  P.H = a->n_kv_heads;
+  P.m = (int)a->budget;
+  P.recent = (int)a->recent;
+  P.sinks = (int)a->sinks;
+  P.row_bytes = (int)(a->head_dim * es);
+  P.zero_tail = a->zero_tail != 0;
+  hipStream_t s = (hipStream_t)stream;
+  {
+    KernelTimer timer("evict_select", s);
+    evict_select_kernel<<<(unsigned)(P.B * P.H), EV_NT, 0, s>>>(P);
+    timer.stop();
+  }
+  NSMOE_TRY(check_launch("evict_select_kernel"));
+  const int rows = P.zero_tail ? (int)P.So : P.m;
+  const bool vec = (bits & 15) == 0;
+  const int64_t items = (int64_t)P.B * rows * P.H * (P.row_bytes / (vec ? 16 : 2));
+  int64_t grid = cdiv(items, EV_MOVE_NT);
+  const int64_t most = 16 * (int64_t)device_cus();
+  if (grid > most) grid = most;
+  KernelTimer timer("evict_move", s);
+  if (vec) evict_move_kernel<u32x4><<<(unsigned)grid, EV_MOVE_NT, 0, s>>>(P, items, rows);
+  else evict_move_kernel<uint16_t><<<(unsigned)grid, EV_MOVE_NT, 0, s>>>(P, items, rows);
+  timer.stop();
+  return check_launch("evict_move_kernel");
+}

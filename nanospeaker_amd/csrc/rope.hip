@@ -1,0 +1,223 @@
+// Rotary positions of query and key heads, forward and backward (bf16, fp16, fp32).
+//
+// Plane j of a head turns by t = position * freq[j] (reference: src/model/rope.py):
+//   y1 = a (x1 cos t - x2 sin t),   y2 = a (x2 cos t + x1 sin t)
+// with x1, x2 dims (j, j + rot / 2) of the head ("rotate half") or (2 j, 2 j + 1)
+// (interleaved), j < rot / 2; dims from rot on pass through.  The frequencies (with whatever
+// stretch a long context asks for folded in) and the amplitude a are the caller's.  The
+// backward is the same kernel with the angle negated: the rotation's transpose.
+//
+// A position may be far (10^6 and more), where an fp32 product position * freq has lost the
+// angle: the product is formed in fp64 in turns, reduced to [-1/2, 1/2] and only then rounded
+// to fp32 (2^-26 of a turn at most), and sin / cos are the library's sincospi.  The rotation
+// itself is fp32 on the widened elements, rounded once to the type.
+//
+// A workgroup takes `tok` consecutive tokens: its threads first make the tok x rot / 2 cosines
+// and sines once, into LDS (they are shared by every head of the token), then stream the
+// heads of q and k, VP planes (two VP-element vectors) a thread and step.  Bound by HBM at
+// long calls (each element read once and written once) and by launch latency at decode ones.
+#include "../../include/nsmoe.h"
+#include "gemm_core.h"
+#include "nsmoe_capi_internal.h"
+
+namespace nsmoe {
+
+constexpr int RP_NT = 256;
+constexpr int RP_MAX_TOK = 16;      // tokens per workgroup
+constexpr int RP_MAX_TRIG = 1024;   // planes x tokens held in LDS, 8 bytes each
+
+struct RopeTensor {
+  const char* src;
+  char* dst;
+  int64_t sb, st, sh;  // input strides in bytes: batch, token, head
+  int64_t db, dt, dh;  // output strides
+};
+
+struct RopeParams {
+  RopeTensor q, k;
+  const int64_t* pos;
+  int64_t pb, pt;  // position strides in elements
+  const double* freq;
+  int64_t rows, T;
+  int nq, nk, D, rot, tok;
+  int copy_tail;  // dims [rot, D) are copied (0: the call is in place)
+  float amp, sign;
+};
+
+template <int DT, int N> struct RopeVec {  // N elements as one (or two) vector accesses
+  typename Elem<DT>::T e[N];
+};
+
+template <int DT, int N>
+__device__ __forceinline__ RopeVec<DT, N> rope_load(const char* p) {
+  RopeVec<DT, N> v;
+  constexpr int B = N * (int)sizeof(v.e[0]), A = B < 16 ? B : 16;
+  __builtin_memcpy(&v, __builtin_assume_aligned(p, A), B);
+  return v;
+}
+template <int DT, int N>
+__device__ __forceinline__ void rope_store(char* p, const RopeVec<DT, N>& v) {
+  constexpr int B = N * (int)sizeof(v.e[0]), A = B < 16 ? B : 16;
+  __builtin_memcpy(__builtin_assume_aligned(p, A), &v, B);
+}
+
+template <int DT, int VP, bool IL>
+__global__ void __launch_bounds__(RP_NT) rope_kernel(RopeParams p) {
+  constexpr int ES = (int)sizeof(typename Elem<DT>::T);
+  __shared__ __attribute__((aligned(16))) float s_cos[RP_MAX_TRIG], s_sin[RP_MAX_TRIG];
+  const int half = p.rot / 2;
+  const int64_t row0 = (int64_t)blockIdx.x * p.tok;
+  const int ntok = (int)min((int64_t)p.tok, p.rows - row0);
+
+  for (int i = threadIdx.x; i < ntok * half; i += RP_NT) {
+    const int t = i / half, j = i - t * half;
+    const int64_t row = row0 + t, b = row / p.T;
+    const double pos = (double)p.pos[b * p.pb + (row - b * p.T) * p.pt];
+    const double turns = pos * (p.freq[j] * 0.15915494309189533577);  // 1 / (2 pi)
+    const float r = (float)(turns - rint(turns));
+    float s, c;
+    sincospif(2.0f * r, &s, &c);
+    s_cos[i] = c * p.amp;
+    s_sin[i] = s * p.amp * p.sign;
+  }
+  __syncthreads();
+
+  // Items of a token: heads x (half / VP rotated vectors pairs, then tail vectors of VP).
+  const int nrot = half / VP;
+  const int ntail = p.copy_tail ? (p.D - p.rot) / VP : 0;
+  const int per_head = nrot + ntail, per_tok = (p.nq + p.nk) * per_head;
+  for (int i = threadIdx.x; i < ntok * per_tok; i += RP_NT) {
+    const int t = i / per_tok, u = i - t * per_tok;
+    int h = u / per_head;
+    const int c = u - h * per_head;
+    const int64_t row = row0 + t, b = row / p.T, tt = row - b * p.T;
+    const bool is_k = h >= p.nq;
+    const RopeTensor& x = is_k ? p.k : p.q;
+    if (is_k) h -= p.nq;
+    const char* src = x.src + b * x.sb + tt * x.st + h * x.sh;
+    char* dst = x.dst + b * x.db + tt * x.dt + h * x.dh;
+    if (c >= nrot) {
+      const int64_t off = (int64_t)(p.rot + (c - nrot) * VP) * ES;
+      rope_store<DT, VP>(dst + off, rope_load<DT, VP>(src + off));
+      continue;
+    }
+    const float* cs = s_cos + t * half + c * VP;
+    const float* sn = s_sin + t * half + c * VP;
+    if constexpr (IL) {
+      const int64_t off = (int64_t)c * 2 * VP * ES;
+      RopeVec<DT, 2 * VP> v = rope_load<DT, 2 * VP>(src + off);
+      float o[2 * VP];
+#pragma unroll
+      for (int e = 0; e < VP; ++e) {
+        const float a = Elem<DT>::to_f(v.e[2 * e]), bb = Elem<DT>::to_f(v.e[2 * e + 1]);
+        o[2 * e] = a * cs[e] - bb * sn[e];
+        o[2 * e + 1] = bb * cs[e] + a * sn[e];
+      }
+      round_to<DT>(o, v.e);
+      rope_store<DT, 2 * VP>(dst + off, v);
+    } else {
+      const int64_t lo = (int64_t)c * VP * ES, hi = lo + (int64_t)half * ES;
+      RopeVec<DT, VP> va = rope_load<DT, VP>(src + lo), vb = rope_load<DT, VP>(src + hi);
+      float oa[VP], ob[VP];
+#pragma unroll
+      for (int e = 0; e < VP; ++e) {
+        const float a = Elem<DT>::to_f(va.e[e]), bb = Elem<DT>::to_f(vb.e[e]);
+        oa[e] = a * cs[e] - bb * sn[e];
+        ob[e] = bb * cs[e] + a * sn[e];
+      }
+      round_to<DT>(oa, va.e);
+      round_to<DT>(ob, vb.e);
+      rope_store<DT, VP>(dst + lo, va);
+      rope_store<DT, VP>(dst + hi, vb);
+    }
+  }
+}
+
+template <int DT, int VP>
+static void rope_run(const RopeParams& P, bool il, unsigned grid, hipStream_t s) {
+  if (il) rope_kernel<DT, VP, true><<<grid, RP_NT, 0, s>>>(P);
+  else rope_kernel<DT, VP, false><<<grid, RP_NT, 0, s>>>(P);
+}
+
+template <int DT>
+static int rope_launch(const RopeParams& P, int vp, bool il, unsigned grid, hipStream_t s) {
+  KernelTimer timer("rope", s);
+  if (vp == 8) rope_run<DT, 8>(P, il, grid, s);
+  else if (vp == 4) rope_run<DT, 4>(P, il, grid, s);
+  else rope_run<DT, 1>(P, il, grid, s);
+  timer.stop();
+  return check_launch("rope_kernel");
+}
+
+}  // namespace nsmoe
+
+using namespace nsmoe;
+
+extern "C" int nsmoe_rope(const nsmoe_rope_args* a, void* stream) {
+  NSMOE_REQUIRE(a, "rope: NULL args");
+  NSMOE_REQUIRE(a->dtype >= DT_BF16 && a->dtype <= DT_F32, "rope: unknown dtype %d", a->dtype);
+  NSMOE_REQUIRE(a->head_dim >= 1 && a->head_dim <= 1024, "rope: head_dim %d (need 1 .. 1024)",
+                a->head_dim);
+  NSMOE_REQUIRE(a->rot_dim >= 2 && a->rot_dim % 2 == 0 && a->rot_dim <= a->head_dim,
+                "rope: rot_dim %d must be even, 2 .. head_dim (%d)", a->rot_dim, a->head_dim);
+  NSMOE_REQUIRE(a->n_q >= 0 && a->n_k >= 0 && a->n_q <= 4096 && a->n_k <= 4096 &&
+                    a->n_q + a->n_k >= 1,
+                "rope: n_q %d and n_k %d (need 0 .. 4096, one of them not 0)", a->n_q, a->n_k);
+  NSMOE_REQUIRE(a->batch >= 0 && a->n_tokens >= 0 && a->batch < INT32_MAX &&
+                    a->n_tokens < INT32_MAX,
+                "rope: bad batch / n_tokens");
+  if (a->batch == 0 || a->n_tokens == 0) return NSMOE_OK;
+  NSMOE_REQUIRE(a->positions && a->freqs && (!a->n_q || (a->q && a->q_out)) &&
+                    (!a->n_k || (a->k && a->k_out)),
+                "rope: NULL pointer");
+  const int es = a->dtype == DT_F32 ? 4 : 2;
+  RopeParams P{};
+  // The widest vectors that the planes, the tail and every address allow: 8 planes a thread
+  // and step (16 bytes of a 16-bit half), 4 where the planes are a multiple of 4 only, else
+  // element by element.
+  uint64_t bits = 0;  // of every address and stride, in bytes
+  auto take = [&](RopeTensor& t, const void* src, void* dst, const int64_t* si, const int64_t* so) {
+    t = RopeTensor{(const char*)src, (char*)dst, si[0] * es, si[1] * es, si[2] * es,
+                   so[0] * es, so[1] * es, so[2] * es};
+    bits |= (uint64_t)src | (uint64_t)dst;
+    for (int i = 0; i < 3; ++i) bits |= (uint64_t)(si[i] * es) | (uint64_t)(so[i] * es);
+  };
+  if (a->n_q) take(P.q, a->q, a->q_out, a->q_stride, a->q_out_stride);
+  if (a->n_k) take(P.k, a->k, a->k_out, a->k_stride, a->k_out_stride);
+  NSMOE_REQUIRE((bits & (uint64_t)(es - 1)) == 0, "rope: misaligned pointer");
+  const bool in_place = (!a->n_q || a->q == a->q_out) && (!a->n_k || a->k == a->k_out);
+  const int half = a->rot_dim / 2, tail = a->head_dim - a->rot_dim;
+  auto fits = [&](int vp) {
+    const uint64_t align = (uint64_t)(vp * es < 16 ? vp * es : 16);
+    return half % vp == 0 && (in_place || tail % vp == 0) && (bits & (align - 1)) == 0;
+  };
+  const int vp = fits(8) ? 8 : fits(4) ? 4 : 1;
+  P.pos = a->positions;
+  P.pb = a->pos_stride[0];
+  P.pt = a->pos_stride[1];
+  P.freq = a->freqs;
+  P.rows = a->batch * a->n_tokens;
+  P.T = a->n_tokens;
+  P.nq = a->n_q;
+  P.nk = a->n_k;
+  P.D = a->head_dim;
+  P.rot = a->rot_dim;
+  P.copy_tail = !in_place;
+  P.amp = a->amplitude;
+  P.sign = a->inverse ? -1.0f : 1.0f;
+  // Tokens per workgroup: one while the call has fewer tokens than two workgroups a CU, then
+  // as many as keep that number, at most 16 and what the LDS table holds.
+  int64_t tok = P.rows / (2 * device_cus());
+  tok = tok < 1 ? 1 : tok > RP_MAX_TOK ? RP_MAX_TOK : tok;
+  if (tok > RP_MAX_TRIG / half) tok = RP_MAX_TRIG / half;
+  P.tok = (int)tok;
+  const int64_t grid = cdiv(P.rows, tok);
+  NSMOE_REQUIRE(grid < INT32_MAX, "rope: grid too large");
+  hipStream_t s = (hipStream_t)stream;
+  const bool il = a->interleaved != 0;
+  switch (a->dtype) {
+    case DT_BF16: return rope_launch<DT_BF16>(P, vp, il, (unsigned)grid, s);
+    case DT_F16: return rope_launch<DT_F16>(P, vp, il, (unsigned)grid, s);
+    default: return rope_launch<DT_F32>(P, vp, il, (unsigned)grid, s);
+  }
+}

@@ -1,0 +1,111 @@
+"""
+Between the head's logits and the choice of a token: penalties for repeated tokens, a bias and
+a grammar mask, in one pass of the library's kernel (nsmoe_penalize_logits).
+"""
+
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+from torch import Tensor
+
+from . import _native as nat
+from .moe_kernel import _DT, _stream, on_device
+
+
+def _vector(name: str, t: Optional[Tensor], n: int, dtype, device) -> Optional[int]:
+    if t is None:
+        return None
+    if t.dtype != dtype or t.shape != (n,) or t.device != device or not t.is_contiguous():
+        raise ValueError(f"penalize_logits: {name} must be a contiguous {dtype} [{n}] on {device}, "
+                         f"got {t.dtype} {tuple(t.shape)} on {t.device}")
+    return t.data_ptr()
+
+
+def _rows(name: str, t: Tensor, b: int, n: int, dtype, device) -> "tuple[int, int]":
+    """(address, row stride) of a [b, n] operand, or of one row [n] or [1, n] for all."""
+    if t.dim() == 1:
+        t = t.unsqueeze(0)
+    if (t.dtype != dtype or t.dim() != 2 or t.shape[0] not in (1, b) or t.shape[1] != n
+            or t.device != device or (t.stride(1) != 1 and n > 1)):
+        raise ValueError(f"penalize_logits: {name} must be {dtype} [{b}, {n}] or [{n}] on {device} "
+                         f"with contiguous rows, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    return t.data_ptr(), t.stride(0) if t.shape[0] == b and b > 1 else 0
+
+
+def penalize_logits(logits: Tensor, history: Optional[Tensor] = None,
+                    lens: Optional[Tensor] = None, *, prompt_lens: Optional[Tensor] = None,
+                    repetition: Optional[Tensor] = None, frequency: Optional[Tensor] = None,
+                    presence: Optional[Tensor] = None, bias: Optional[Tensor] = None,
+                    mask: Optional[Tensor] = None, out: Optional[Tensor] = None) -> Tensor:
+    """
+    The logits [batch, vocab] (bf16, fp16 or fp32) with, in this order,
+
+      * `repetition` [batch] fp32: tokens of the row's history divided by it where positive and
+        multiplied by it where negative (1: no change; it must be positive);
+      * `frequency` and `presence` [batch] fp32: frequency times the token's count and, where
+        the count is not 0, presence subtracted; counted over the history after its first
+        `prompt_lens` [batch] int32 tokens (all of it without);
+      * `bias` fp32 [batch, vocab] or [vocab] added;
+      * `mask` int32 [batch, ceil(vocab / 32)] or [ceil(vocab / 32)]: -inf where bit v % 32 of
+        word v / 32 is 0, whatever the logit was.  A row that allows nothing is all -inf.
+
+    history: int64 [batch, n], of which row b holds lens[b] (int32; n without) tokens; ids
+    outside the vocabulary count nothing, so -1 may pad.  Computed in fp32 and rounded once, to
+    the logits' type or to that of `out` (that type or fp32; logits itself writes in place).
+    """
+    if logits.dim() != 2 or not logits.is_cuda or logits.dtype not in _DT:
+        raise ValueError("penalize_logits: logits must be a bf16, fp16 or fp32 [batch, vocab] GPU "
+                         f"tensor, got {logits.dtype} {tuple(logits.shape)} on {logits.device}")
+    b, v = logits.shape
+    dev = logits.device
+    if v > 1 and logits.stride(1) != 1:
+        raise ValueError("penalize_logits: the rows of logits must be contiguous")
+    if out is None:
+        out = torch.empty((b, v), dtype=logits.dtype, device=dev)
+    elif (out.shape != (b, v) or out.device != dev or out.dtype not in (logits.dtype, torch.float32)
+          or (v > 1 and out.stride(1) != 1) or (b > 1 and out.stride(0) < v)):
+        raise ValueError(f"penalize_logits: out must be [{b}, {v}] with contiguous rows of the "
+                         f"logits' type or fp32 on {dev}, got {out.dtype} {tuple(out.shape)}")
+    elif out is not logits and out.numel() and _overlap(out, logits) and not (
+            out.data_ptr() == logits.data_ptr() and out.dtype == logits.dtype
+            and (b == 1 or out.stride(0) == logits.stride(0))):
+        raise ValueError("penalize_logits: out overlaps logits without being them")
+    f = {}
+    if history is None:
+        if any(t is not None for t in (repetition, frequency, presence, lens, prompt_lens)):
+            raise ValueError("penalize_logits: penalties and lengths need a history")
+    else:
+        if history.dim() != 2:
+            raise ValueError(f"penalize_logits: history {tuple(history.shape)}, expected [{b}, n]")
+        n = history.shape[1]
+        if history.shape[0] != b:
+            raise ValueError(f"penalize_logits: history of {history.shape[0]} rows for {b}")
+        p, s = _rows("history", history, b, n, torch.int64, dev)
+        f.update(history=p if n else None, history_stride=s, history_cap=n)
+    f32 = torch.float32
+    f.update(lens=_vector("lens", lens, b, torch.int32, dev),
+             prompt_lens=_vector("prompt_lens", prompt_lens, b, torch.int32, dev),
+             repetition=_vector("repetition", repetition, b, f32, dev),
+             frequency=_vector("frequency", frequency, b, f32, dev),
+             presence=_vector("presence", presence, b, f32, dev))
+    if bias is not None:
+        f["bias"], f["bias_stride"] = _rows("bias", bias, b, v, f32, dev)
+    if mask is not None:
+        f["mask"], f["mask_stride"] = _rows("mask", mask, b, (v + 31) // 32, torch.int32, dev)
+    a = nat.LogitsArgs(dtype=_DT[logits.dtype], out_dtype=_DT[out.dtype], batch=b, vocab=v,
+                       logits=logits.data_ptr(), out=out.data_ptr(),
+                       logits_stride=logits.stride(0), out_stride=out.stride(0), **f)
+    with on_device(dev):
+        nat.check(nat.lib().nsmoe_penalize_logits(a, _stream(dev.index)), "nsmoe_penalize_logits")
+    return out
+
+
+def _overlap(a: Tensor, b: Tensor) -> bool:
+    """Whether the address ranges of two 2-d tensors with contiguous rows meet."""
+    def span(t):
+        last = (t.shape[0] - 1) * t.stride(0) + t.shape[1]
+        return t.data_ptr(), t.data_ptr() + last * t.element_size()
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a0 < b1 and b0 < a1

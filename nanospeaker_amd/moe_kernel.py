@@ -101,6 +101,17 @@ def _stream(device_index: "int | None" = None) -> int:
     return _raw_stream(device_index)
 
 
+def on_device(device):
+    """A context in which `device` is the current one (nothing to do when it already is): a
+    launch goes to the current device, whatever device its stream belongs to."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return _HERE
+    return torch.cuda.device(device)
+
+
+_HERE = nullcontext()
+
+
 def _p(t: Optional[Tensor]) -> Optional[int]:
     return None if t is None or t.numel() == 0 else t.data_ptr()
 
