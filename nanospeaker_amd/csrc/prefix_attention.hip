@@ -36,6 +36,7 @@ namespace nsmoe {
 
 constexpr int PA_NT = 256;
 constexpr float PA_NONE = -INFINITY;
+constexpr bool PA_SPLIT_MANY = false;
 
 struct PrefixAttnParams {
   const uint16_t *q, *kp, *vp, *k, *v;
@@ -43,17 +44,18 @@ struct PrefixAttnParams {
   int64_t kpt, kph, vpt, vph;  // prefix: row, head
   int64_t kb, kt, kh, vb, vt, vh;
   const int32_t* lens;
-  float* part_o;   // [slots][rows][D]
-  float2* part_ml; // [slots][rows]: log2-scaled maximum, sum
+  float* part_o;   // [rows][slots][D]
+  float2* part_ml; // [rows][slots]: log2-scaled maximum, sum
   float* score;    // [B, Hkv, n G, spad] log2-scaled scores of the own rows, or NULL
   uint16_t* out;   // [rows, D]
   float* lse;      // [rows] or NULL
   const float* w_in;
   float* w_out;    // [B, Hkv, S]
   int B, n, P, S, Hq, Hkv, G, window, spad;
-  int np, ns;      // parts of the prefix and of each own cache
-  int rbp, rbs;    // column blocks of a prefix part and of an own part
-  int items_p;     // workgroups of the prefix (before the own ones)
+  int np, ns;            // parts of the prefix and of each own cache: a row's slots
+  int chunk_p, chunk_s;  // keys per part
+  int rbp, rbs;          // column blocks of a prefix part and of an own part
+  int items_p;           // workgroups of the prefix (before the own ones)
   float scale_log2;
 };
 
@@ -68,17 +70,21 @@ struct PartJob {
   int64_t kt, vt;         // row strides
   int hk, b;              // b < 0: the prefix
   int col0, cols;         // first column, and how many columns there are in all
-  int split, splits, slot;
+  int key0, key1;         // the part's keys
+  int slot;
 };
 
 __device__ __forceinline__ PartJob pa_job(const PrefixAttnParams& p, int item, bool own,
                                           int width) {
   PartJob j;
   if (!own) {
-    j.split = item % p.np;
-    item /= p.np;
+    // Column blocks of one run of keys follow each other and sit on one XCD: they read the
+    // same keys and values from its L2.
+    item = xcd_remap(item, p.items_p);
     const int rb = item % p.rbp;
-    j.hk = item / p.rbp;
+    item /= p.rbp;
+    const int split = item % p.np;
+    j.hk = item / p.np;
     j.b = -1;
     j.k = p.kp + j.hk * p.kph;
     j.v = p.vp + j.hk * p.vph;
@@ -86,23 +92,26 @@ __device__ __forceinline__ PartJob pa_job(const PrefixAttnParams& p, int item, b
     j.vt = p.vpt;
     j.col0 = rb * width;
     j.cols = p.B * p.n * p.G;
-    j.splits = p.np;
-    j.slot = j.split;
+    j.key0 = split * p.chunk_p;
+    j.key1 = j.key0 + p.chunk_p;
+    j.slot = split;
   } else {
-    j.split = item % p.ns;
-    item /= p.ns;
+    // Parts in the order of their keys: the ones that short sequences leave empty come last.
+    j.hk = item % p.Hkv;
+    item /= p.Hkv;
     const int rb = item % p.rbs;
     item /= p.rbs;
-    j.hk = item % p.Hkv;
-    j.b = item / p.Hkv;
+    j.b = item % p.B;
+    const int split = item / p.B;
     j.k = p.k + j.b * p.kb + j.hk * p.kh;
     j.v = p.v + j.b * p.vb + j.hk * p.vh;
     j.kt = p.kt;
     j.vt = p.vt;
     j.col0 = rb * width;
     j.cols = p.n * p.G;
-    j.splits = p.ns;
-    j.slot = p.np + j.split;
+    j.key0 = split * p.chunk_s;
+    j.key1 = j.key0 + p.chunk_s;
+    j.slot = p.np + split;
   }
   return j;
 }
@@ -204,18 +213,14 @@ __device__ __forceinline__ void pa_load_cols(const PrefixAttnParams& p, const Pa
   lo = min(lo, hi);  // nothing seen: an empty range
 }
 
-// One tile of KB * 16 keys from key0 on: scores, online softmax, P V.  Kt / Vt: the tile's rows
-// in LDS.  `score`: where to leave this lane's column's scaled scores (its tile's key 0), or
-// NULL per block.
+// A tile of KB * 16 keys from key0 on, in three steps.  Scores: S^T = K Q^T from the K rows in
+// LDS; lane (g, l16) gets keys 16 kb + 4 g + e of column l16.
 template <int DT, int D, int NB, int KB>
-__device__ __forceinline__ void pa_tile(const PaCols<DT, D, NB>& w, PaState<D, NB>& st,
-                                        const char* Kt, const char* Vt, int key0, float c,
-                                        int lane, float* const (&score)[NB]) {
+__device__ __forceinline__ void pa_scores(const PaCols<DT, D, NB>& w, const char* Kt, int lane,
+                                          f32x4 (&s)[KB][NB]) {
   using M = Mma<DT>;
-  using Frag = typename M::Frag;
   constexpr int RB = 2 * D;  // bytes per row
   const int l16 = lane & 15, g = lane >> 4;
-  f32x4 s[KB][NB];
 #pragma unroll
   for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
@@ -225,10 +230,19 @@ __device__ __forceinline__ void pa_tile(const PaCols<DT, D, NB>& w, PaState<D, N
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
       const int r = 16 * kb + l16;
-      const Frag kf = M::load(Kt + r * RB + (((4 * ks + g) ^ pa_swz<D>(r)) << 4));
+      const typename M::Frag kf = M::load(Kt + r * RB + (((4 * ks + g) ^ pa_swz<D>(r)) << 4));
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) M::run(s[kb][nb], kf, w.q[nb][ks]);
     }
+}
+
+// Masks, then turns the scores into probabilities against the running maximum.  `score`: where
+// to leave this lane's column's scaled scores (the tile's key 0), or NULL per block.
+template <int DT, int D, int NB, int KB>
+__device__ __forceinline__ void pa_softmax(const PaCols<DT, D, NB>& w, PaState<D, NB>& st,
+                                           f32x4 (&s)[KB][NB], int key0, float c, int lane,
+                                           float* const (&score)[NB]) {
+  const int g = lane >> 4;
   // Keys outside a column's range: one select per score, on tiles that cross some edge only.
   bool edge = false;
 #pragma unroll
@@ -281,16 +295,34 @@ __device__ __forceinline__ void pa_tile(const PaCols<DT, D, NB>& w, PaState<D, N
       }
     st.l[nb] += sum;
   }
-  // O^T += V^T P^T, 32 keys at a time: slot 8 g + e is key 4 g + e, slot 8 g + 4 + e key
-  // 16 + 4 g + e, of P and of V alike.
+}
+
+// O^T += V^T P^T, 32 keys at a time: slot 8 g + e is key 4 g + e, slot 8 g + 4 + e key
+// 16 + 4 g + e, of P and of V alike.  With SPLIT the part of each probability that its rounding
+// to the type leaves behind is multiplied too, rounded in its turn: 2^-16 of it is lost
+// instead of 2^-9 (bf16).
+template <int DT, int D, int NB, int KB, bool SPLIT>
+__device__ __forceinline__ void pa_values(PaState<D, NB>& st, const f32x4 (&s)[KB][NB],
+                                          const char* Vt, int lane) {
+  using M = Mma<DT>;
+  using Frag = typename M::Frag;
+  constexpr int RB = 2 * D;
+  const int l16 = lane & 15, g = lane >> 4;
 #pragma unroll
   for (int ks = 0; ks < KB / 2; ++ks) {
-    Frag pf[NB];
+    Frag pf[NB], pr[NB];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
       const f32x4 a = s[2 * ks][nb], b = s[2 * ks + 1][nb];
       pf[nb].v = u32x4{pack2<DT>(a[0], a[1]), pack2<DT>(a[2], a[3]), pack2<DT>(b[0], b[1]),
                        pack2<DT>(b[2], b[3])};
+      if constexpr (SPLIT) {
+        auto rest = [&](float x, float y, uint32_t hi) {
+          return pack2<DT>(x - unpack2<DT>(hi, 0), y - unpack2<DT>(hi, 1));
+        };
+        pr[nb].v = u32x4{rest(a[0], a[1], pf[nb].v[0]), rest(a[2], a[3], pf[nb].v[1]),
+                         rest(b[0], b[1], pf[nb].v[2]), rest(b[2], b[3], pf[nb].v[3])};
+      }
     }
     const int ra = 32 * ks + 4 * g + (l16 >> 2), rb = ra + 16;
     const int sub = (l16 & 3) >> 1, within = 8 * (l16 & 1);
@@ -302,7 +334,10 @@ __device__ __forceinline__ void pa_tile(const PaCols<DT, D, NB>& w, PaState<D, N
       Frag vf;
       vf.v = u32x4{lo.x, lo.y, hi.x, hi.y};
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) M::run(st.o[db][nb], vf, pf[nb]);
+      for (int nb = 0; nb < NB; ++nb) {
+        M::run(st.o[db][nb], vf, pf[nb]);
+        if constexpr (SPLIT) M::run(st.o[db][nb], vf, pr[nb]);
+      }
     }
   }
 }
@@ -318,19 +353,37 @@ __device__ __forceinline__ void pa_clear(PaState<D, NB>& st) {
   }
 }
 
-// LDS-DMA of `rows` rows from row key0 on of one of K / V into LDS at `dst`, rows outside
-// [lo, hi) as zeros (what lies there was never written, and 0 * NaN is NaN).  A copy is 1 KiB.
-template <int D>
-__device__ __forceinline__ void pa_copy(const uint16_t* base, int64_t stride, int row, int key0,
-                                        int lo, int hi, uint32_t dst, int lane) {
-  constexpr int CPR = D / 8;  // chunks per row
-  const int r = row + lane / CPR;
-  const int c = (lane % CPR) ^ pa_swz<D>(r);
-  const int key = key0 + r;
-  const uint16_t* src = base + (int64_t)key * stride + c * 8;
-  if (key < lo || key >= hi) src = (const uint16_t*)((const char*)g_zero_kib + lane * 16);
-  async_copy16_to(src, dst);
-}
+// LDS-DMA copies of a wave for one of K / V: N copies of 1 KiB (1024 / 2 D rows each) from row
+// `row0` of a tile on, into LDS at `dst` plus 1 KiB each.  Rows outside [lo, hi) become zeros:
+// what lies there was never written, and 0 * NaN is NaN.
+template <int D, int N>
+struct PaCopy {
+  const uint16_t* src[N];  // this lane's chunk in tile 0
+  int row[N];
+  int64_t stride;
+
+  __device__ __forceinline__ void set(const uint16_t* base, int64_t st, int row0, int lane) {
+    constexpr int CPR = D / 8, RPC = 64 / CPR;  // chunks per row, rows per copy
+    stride = st;
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      row[u] = row0 + u * RPC + lane / CPR;
+      src[u] = base + row[u] * st + ((lane % CPR) ^ pa_swz<D>(row[u])) * 8;
+    }
+  }
+  __device__ __forceinline__ void issue(int key0, int keys, int lo, int hi, uint32_t dst,
+                                        int lane) const {
+    const int64_t off = (int64_t)key0 * stride;
+    const bool whole = key0 >= lo && key0 + keys <= hi;  // uniform
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      const uint16_t* s = src[u] + off;
+      if (!whole && (key0 + row[u] < lo || key0 + row[u] >= hi))
+        s = (const uint16_t*)((const char*)g_zero_kib + lane * 16);
+      async_copy16_to(s, dst + u * 1024);
+    }
+  }
+};
 
 __device__ __forceinline__ uint32_t pa_lds(const char* p) {
   return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)p;
@@ -338,38 +391,26 @@ __device__ __forceinline__ uint32_t pa_lds(const char* p) {
 
 template <int D> struct PaGeo {
   static constexpr int FEW_KEYS = 32;
-  static constexpr int FEW_STAGES = D == 64 ? 3 : 2;
-  static constexpr int FEW_TILE = FEW_KEYS * 2 * D;                    // bytes of K or V
-  static constexpr int FEW_LDS = 4 * FEW_STAGES * 2 * FEW_TILE;
+  static constexpr int FEW_TILE = FEW_KEYS * 2 * D;  // bytes of K or V
+  static constexpr int FEW_LDS = 4 * 2 * FEW_TILE;   // 32 or 64 KiB
   static constexpr int MANY_KEYS = 64;
   static constexpr int MANY_STAGES = D == 64 ? 3 : 2;
   static constexpr int MANY_TILE = MANY_KEYS * 2 * D;
-  static constexpr int MANY_LDS = MANY_STAGES * 2 * MANY_TILE;
+  static constexpr int MANY_LDS = MANY_STAGES * 2 * MANY_TILE;  // 48 or 64 KiB
 };
-
-// The split's run of key tiles: [lo, hi) cut into whole tiles from lo's tile on, dealt evenly.
-__device__ __forceinline__ void pa_range(int lo, int hi, int tile, const PartJob& j, int& t0,
-                                         int& t1) {
-  const int a = lo / tile, b = hi > lo ? (hi + tile - 1) / tile : a;
-  const int per = (b - a + j.splits - 1) / j.splits;
-  t0 = min(b, a + j.split * per);
-  t1 = min(b, t0 + per);
-}
 
 template <int DT, int D, int NB>
 __device__ void pa_few(const PrefixAttnParams& p, const PartJob& j, char* lds) {
   using Geo = PaGeo<D>;
-  constexpr int KEYS = Geo::FEW_KEYS, ST = Geo::FEW_STAGES, TILE = Geo::FEW_TILE;
-  constexpr int RPC = 1024 / (2 * D);   // rows per copy
-  constexpr int NC = KEYS / RPC;        // copies of one of K / V per tile
+  constexpr int KEYS = Geo::FEW_KEYS, TILE = Geo::FEW_TILE, KB = KEYS / 16;
+  constexpr int NC = TILE / 1024;  // copies of one of K / V per tile
   const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   PaCols<DT, D, NB> w;
-  int lo, hi, t0, t1;
+  int lo, hi;
   pa_load_cols<DT, D, NB>(p, j, j.col0, lane, w, lo, hi);
-  lo = __builtin_amdgcn_readfirstlane(lo);
-  hi = __builtin_amdgcn_readfirstlane(hi);
-  pa_range(lo, hi, KEYS, j, t0, t1);
+  lo = __builtin_amdgcn_readfirstlane(max(lo, j.key0));
+  hi = __builtin_amdgcn_readfirstlane(min(hi, j.key1));
   float* score[NB];
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
@@ -377,97 +418,90 @@ __device__ void pa_few(const PrefixAttnParams& p, const PartJob& j, char* lds) {
     score[nb] = p.score && j.b >= 0 && col < j.cols
                     ? p.score + (((int64_t)j.b * p.Hkv + j.hk) * j.cols + col) * p.spad
                     : nullptr;
+    // Padding columns see nothing and ask for no mask.
+    if (col >= j.cols) w.first[nb] = 0, w.last[nb] = INT32_MAX;
   }
-  // The columns' ranges may start late or end early: rows of a tile that no column sees are
-  // not copied.  Padding columns see nothing and ask for no mask.
-#pragma unroll
-  for (int nb = 0; nb < NB; ++nb)
-    if (j.col0 + 16 * nb + l16 >= j.cols) w.first[nb] = 0, w.last[nb] = INT32_MAX;
-
-  char* ring = lds + wave * ST * 2 * TILE;
-  const uint32_t ring0 = pa_lds(ring);
-  auto issue = [&](int t, int stage) {
-    const uint32_t dst = ring0 + (uint32_t)(stage * 2 * TILE);
-#pragma unroll
-    for (int u = 0; u < NC; ++u)
-      pa_copy<D>(j.k, j.kt, u * RPC, t * KEYS, lo, hi, dst + u * 1024, lane);
-#pragma unroll
-    for (int u = 0; u < NC; ++u)
-      pa_copy<D>(j.v, j.vt, u * RPC, t * KEYS, lo, hi, dst + TILE + u * 1024, lane);
-  };
+  // One buffer each for K and V, a wave's own: the next tile's K is copied from when this
+  // one's scores are done, its V from when this one's product is.  What hides the copies'
+  // latency is the other waves of the CU (8 to 16, each with 8 or 16 KiB of tile).
   PaState<D, NB> st;
   pa_clear(st);
-  // Tiles wave, wave + 4, ...; ST - 1 of them in flight ahead of the one being multiplied.
-#pragma unroll
-  for (int u = 0; u < ST - 1; ++u)
-    if (t0 + wave + 4 * u < t1) issue(t0 + wave + 4 * u, u);
-  int stage = 0;
-  for (int t = t0 + wave; t < t1; t += 4) {
-    // The tile ST - 1 ahead goes into the stage that the previous turn has read: its LDS
-    // reads have to be done (their results in registers) before the copy may land.
+  char* Kt = lds + wave * 2 * TILE;
+  char* Vt = Kt + TILE;
+  const uint32_t kd = pa_lds(Kt), vd = kd + TILE;
+  PaCopy<D, NC> ck, cv;
+  ck.set(j.k, j.kt, 0, lane);
+  cv.set(j.v, j.vt, 0, lane);
+  int t = lo / KEYS + wave;
+  const int t1 = hi > lo ? (hi + KEYS - 1) / KEYS : 0;
+  if (t < t1) {
+    ck.issue(t * KEYS, KEYS, lo, hi, kd, lane);
+    cv.issue(t * KEYS, KEYS, lo, hi, vd, lane);
+  }
+  for (; t < t1; t += 4) {
+    f32x4 s[KB][NB];
+    wait_vmcnt<NC>();  // this tile's K; its V stays in flight
     asm volatile("" ::: "memory");
-    wait_lgkm0();
-    const int ahead = t + 4 * (ST - 1);
-    if (ahead < t1) issue(ahead, (stage + ST - 1) % ST);
-    // this tile's copies; those of the tiles behind it stay in flight
-    const int later = min(ST - 1, (t1 - 1 - t) / 4);
-    if (later == 0) wait_vmcnt<0>();
-    else if (later == 1) wait_vmcnt<2 * NC>();
-    else wait_vmcnt<4 * NC>();
+    pa_scores<DT, D, NB, KB>(w, Kt, lane, s);
     asm volatile("" ::: "memory");
-    const char* tile = ring + stage * 2 * TILE;
+    wait_lgkm0();      // K has been read
+    const bool more = t + 4 < t1;
+    if (more) ck.issue((t + 4) * KEYS, KEYS, lo, hi, kd, lane);
     float* sc[NB];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) sc[nb] = score[nb] ? score[nb] + t * KEYS : nullptr;
-    pa_tile<DT, D, NB, KEYS / 16>(w, st, tile, tile + TILE, t * KEYS, p.scale_log2, lane, sc);
-    stage = stage + 1 == ST ? 0 : stage + 1;
+    pa_softmax<DT, D, NB, KB>(w, st, s, t * KEYS, p.scale_log2, lane, sc);
+    if (more) wait_vmcnt<NC>();  // this tile's V; the next K stays in flight
+    else wait_vmcnt<0>();
+    asm volatile("" ::: "memory");
+    pa_values<DT, D, NB, KB, DT == DT_BF16>(st, s, Vt, lane);
+    asm volatile("" ::: "memory");
+    wait_lgkm0();      // V has been read
+    if (more) cv.issue((t + 4) * KEYS, KEYS, lo, hi, vd, lane);
   }
-  wait_vmcnt<0>();
 
-  // Join the four waves: every wave's maximum, sum and output through LDS.
-  __syncthreads();
-  constexpr int W = 16 * NB;
-  float* s_o = (float*)lds;                    // [4][W][D]
-  float* s_m = (float*)(lds + 4 * W * D * 4);  // [4][W]
-  float* s_l = s_m + 4 * W;                    // [4][W]
+  // Join the four waves through LDS, 16 columns at a time.
+  float* s_o = (float*)lds;                     // [4][16][D]
+  float* s_m = (float*)(lds + 4 * 16 * D * 4);  // [4][16]
+  float* s_l = s_m + 4 * 16;                    // [4][16]
+  const int slots = p.np + p.ns;
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
     float l = st.l[nb];
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
-    const int col = 16 * nb + l16;
+    __syncthreads();
     if (g == 0) {
-      s_m[wave * W + col] = st.m[nb];
-      s_l[wave * W + col] = l;
+      s_m[wave * 16 + l16] = st.m[nb];
+      s_l[wave * 16 + l16] = l;
     }
 #pragma unroll
     for (int db = 0; db < D / 16; ++db)
-      *(f32x4*)(s_o + (wave * W + col) * D + 16 * db + 4 * g) = st.o[db][nb];
-  }
-  __syncthreads();
-  const int64_t rows = (int64_t)p.B * p.n * p.Hq;
-  for (int i = threadIdx.x; i < W * (D / 4); i += PA_NT) {
-    const int col = i / (D / 4), d = (i % (D / 4)) * 4;
-    const Column c = pa_column(p, j, j.col0 + col);
-    if (c.row < 0) continue;
-    float m = PA_NONE;
+      *(f32x4*)(s_o + (wave * 16 + l16) * D + 16 * db + 4 * g) = st.o[db][nb];
+    __syncthreads();
+    for (int i = threadIdx.x; i < 16 * (D / 4); i += PA_NT) {
+      const int col = i / (D / 4), d = (i % (D / 4)) * 4;
+      const Column c = pa_column(p, j, j.col0 + 16 * nb + col);
+      if (c.row < 0) continue;
+      float m = PA_NONE;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) m = fmaxf(m, s_m[k * W + col]);
-    if (c.last < c.first) m = PA_NONE;
-    f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    float l = 0.0f;
-    if (m != PA_NONE) {
+      for (int k = 0; k < 4; ++k) m = fmaxf(m, s_m[k * 16 + col]);
+      const int64_t at = c.row * slots + j.slot;
+      f32x4 o = {0.f, 0.f, 0.f, 0.f};
+      float sum = 0.0f;
+      if (m != PA_NONE) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float mk = s_m[k * W + col];
-        if (mk == PA_NONE) continue;
-        const float f = __builtin_amdgcn_exp2f((mk - m) * p.scale_log2);
-        l += s_l[k * W + col] * f;
-        o += *(const f32x4*)(s_o + (k * W + col) * D + d) * f;
+        for (int k = 0; k < 4; ++k) {
+          const float mk = s_m[k * 16 + col];
+          if (mk == PA_NONE) continue;
+          const float f = __builtin_amdgcn_exp2f((mk - m) * p.scale_log2);
+          sum += s_l[k * 16 + col] * f;
+          o += *(const f32x4*)(s_o + (k * 16 + col) * D + d) * f;
+        }
+        *(f32x4*)(p.part_o + at * D + d) = o;
       }
-      *(f32x4*)(p.part_o + (j.slot * rows + c.row) * D + d) = o;
+      if (d == 0) p.part_ml[at] = make_float2(m * p.scale_log2, sum);
     }
-    if (d == 0) p.part_ml[j.slot * rows + c.row] = make_float2(m * p.scale_log2, l);
   }
 }
 
@@ -475,22 +509,22 @@ template <int DT, int D, int NB>
 __device__ void pa_many(const PrefixAttnParams& p, const PartJob& j, char* lds) {
   using Geo = PaGeo<D>;
   constexpr int KEYS = Geo::MANY_KEYS, ST = Geo::MANY_STAGES, TILE = Geo::MANY_TILE;
-  constexpr int RPC = 1024 / (2 * D);
-  constexpr int NC = KEYS / RPC / 4;  // copies of one of K / V per tile and wave
+  constexpr int KB = KEYS / 16;
+  constexpr int NC = TILE / 1024 / 4;  // copies of one of K / V per tile and wave
   const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  __shared__ int s_lo[4], s_hi[4];
   PaCols<DT, D, NB> w;
-  int lo, hi, t0, t1;
+  int lo, hi;
   const int c0 = j.col0 + wave * 16 * NB;
   pa_load_cols<DT, D, NB>(p, j, c0, lane, w, lo, hi);
-  if (lane == 0) s_lo[wave] = hi > lo ? lo : INT32_MAX, s_hi[wave] = hi;
+  int* s_lo = (int*)lds;  // [4], then s_hi[4]
+  if (lane == 0) s_lo[wave] = hi > lo ? lo : INT32_MAX, s_lo[4 + wave] = hi;
   __syncthreads();
   lo = min(min(s_lo[0], s_lo[1]), min(s_lo[2], s_lo[3]));
-  hi = max(max(s_hi[0], s_hi[1]), max(s_hi[2], s_hi[3]));
-  lo = __builtin_amdgcn_readfirstlane(min(lo, hi));
-  hi = __builtin_amdgcn_readfirstlane(hi);
-  pa_range(lo, hi, KEYS, j, t0, t1);
+  hi = max(max(s_lo[4], s_lo[5]), max(s_lo[6], s_lo[7]));
+  lo = __builtin_amdgcn_readfirstlane(max(lo, j.key0));
+  hi = __builtin_amdgcn_readfirstlane(min(hi, j.key1));
+  __syncthreads();  // before the first copies land there
   float* score[NB];
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
@@ -500,22 +534,19 @@ __device__ void pa_many(const PrefixAttnParams& p, const PartJob& j, char* lds) 
                     : nullptr;
     if (col >= j.cols) w.first[nb] = 0, w.last[nb] = INT32_MAX;
   }
-  const uint32_t lds0 = pa_lds(lds);
+  const uint32_t lds0 = pa_lds(lds) + (uint32_t)(wave * NC * 1024);
+  PaCopy<D, NC> ck, cv;
+  constexpr int ROWS = KEYS / 4;  // rows that a wave copies
+  ck.set(j.k, j.kt, wave * ROWS, lane);
+  cv.set(j.v, j.vt, wave * ROWS, lane);
   auto issue = [&](int t, int stage) {
     const uint32_t dst = lds0 + (uint32_t)(stage * 2 * TILE);
-#pragma unroll
-    for (int u = 0; u < NC; ++u) {
-      const int cp = wave * NC + u;
-      pa_copy<D>(j.k, j.kt, cp * RPC, t * KEYS, lo, hi, dst + cp * 1024, lane);
-    }
-#pragma unroll
-    for (int u = 0; u < NC; ++u) {
-      const int cp = wave * NC + u;
-      pa_copy<D>(j.v, j.vt, cp * RPC, t * KEYS, lo, hi, dst + TILE + cp * 1024, lane);
-    }
+    ck.issue(t * KEYS, KEYS, lo, hi, dst, lane);
+    cv.issue(t * KEYS, KEYS, lo, hi, dst + TILE, lane);
   };
   PaState<D, NB> st;
   pa_clear(st);
+  const int t0 = hi > lo ? lo / KEYS : 0, t1 = hi > lo ? (hi + KEYS - 1) / KEYS : 0;
 #pragma unroll
   for (int u = 0; u < ST - 1; ++u)
     if (t0 + u < t1) issue(t0 + u, u);
@@ -525,18 +556,21 @@ __device__ void pa_many(const PrefixAttnParams& p, const PartJob& j, char* lds) 
     if (ST == 3 && t + 1 < t1) wait_vmcnt<2 * NC>();
     else wait_vmcnt<0>();
     asm volatile("" ::: "memory");
-    wait_lgkm0();  // this wave's LDS reads of the stage that is copied into next
+    wait_lgkm0();   // this wave's LDS reads of the stage that is copied into next
     barrier_dma();  // every wave's copies of tile t; every wave done with tile t - 1
     if (t + ST - 1 < t1) issue(t + ST - 1, (stage + ST - 1) % ST);
     const char* tile = lds + stage * 2 * TILE;
     float* sc[NB];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) sc[nb] = score[nb] ? score[nb] + t * KEYS : nullptr;
-    pa_tile<DT, D, NB, KEYS / 16>(w, st, tile, tile + TILE, t * KEYS, p.scale_log2, lane, sc);
+    f32x4 s[KB][NB];
+    pa_scores<DT, D, NB, KB>(w, tile, lane, s);
+    pa_softmax<DT, D, NB, KB>(w, st, s, t * KEYS, p.scale_log2, lane, sc);
+    pa_values<DT, D, NB, KB, PA_SPLIT_MANY && DT == DT_BF16>(st, s, tile + TILE, lane);
     stage = stage + 1 == ST ? 0 : stage + 1;
   }
   wait_vmcnt<0>();
-  const int64_t rows = (int64_t)p.B * p.n * p.Hq;
+  const int slots = p.np + p.ns;
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
     float l = st.l[nb];
@@ -544,175 +578,247 @@ __device__ void pa_many(const PrefixAttnParams& p, const PartJob& j, char* lds) 
     l += __shfl_xor(l, 32);
     const Column c = pa_column(p, j, c0 + 16 * nb + l16);
     if (c.row < 0) continue;
-    const float m = c.last < c.first ? PA_NONE : st.m[nb];
-    if (g == 0) p.part_ml[j.slot * rows + c.row] = make_float2(m * p.scale_log2, l);
-    if (m == PA_NONE) continue;
-    float* dst = p.part_o + (j.slot * rows + c.row) * D + 4 * g;
+    const int64_t at = c.row * slots + j.slot;
+    if (g == 0) p.part_ml[at] = make_float2(st.m[nb] * p.scale_log2, l);
+    if (st.m[nb] == PA_NONE) continue;
+    float* dst = p.part_o + at * D + 4 * g;
 #pragma unroll
     for (int db = 0; db < D / 16; ++db) *(f32x4*)(dst + 16 * db) = st.o[db][nb];
   }
 }
 
-// Forms: 0, 1 few with 1 or 2 column blocks; 2, 3 many with 1 or 2 per wave.
-constexpr int PA_WIDTH[4] = {16, 32, 64, 128};
+// Forms: 0, 1 few with 1 or 2 column blocks; 2, 3, 4 many with 1, 2 or 3 per wave.
+constexpr int PA_FORMS = 5;
+constexpr int PA_WIDTH[PA_FORMS] = {16, 32, 64, 128, 192};
 
 template <int DT, int D, int FORM>
-__global__ void __launch_bounds__(PA_NT) prefix_part_kernel(PrefixAttnParams p, int own) {
-  extern __shared__ __attribute__((aligned(1024))) char lds[];
-  const PartJob j = pa_job(p, (int)blockIdx.x, own != 0, PA_WIDTH[FORM]);
+__device__ __forceinline__ void pa_part(const PrefixAttnParams& p, int item, bool own, char* lds) {
+  const PartJob j = pa_job(p, item, own, PA_WIDTH[FORM]);
   if constexpr (FORM < 2) pa_few<DT, D, FORM + 1>(p, j, lds);
   else pa_many<DT, D, FORM - 1>(p, j, lds);
 }
 
-// log2 of a row's whole sum of exponentials, from its parts; -inf for a row that saw nothing.
-__device__ __forceinline__ void pa_total(const PrefixAttnParams& p, int64_t row, int64_t rows,
-                                         float& m, float& l) {
-  const int slots = p.np + p.ns;
-  m = PA_NONE;
-  for (int s = 0; s < slots; ++s) m = fmaxf(m, p.part_ml[s * rows + row].x);
-  l = 0.0f;
-  if (m == PA_NONE) return;
-  for (int s = 0; s < slots; ++s) {
-    const float2 ml = p.part_ml[s * rows + row];
-    if (ml.x != PA_NONE) l += ml.y * __builtin_amdgcn_exp2f(ml.x - m);
+// The parts of the prefix (form FP) and, behind them, those of the own caches (form FS) in one
+// launch: the first are bound by arithmetic under a batch, the second by HBM.  FP or FS -1:
+// none of that kind.
+template <int DT, int D, int FP, int FS>
+__global__ void __launch_bounds__(PA_NT, 2) prefix_part_kernel(PrefixAttnParams p) {
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
+  const int item = (int)blockIdx.x;
+  if constexpr (FP >= 0) {
+    if (FS < 0 || item < p.items_p) {
+      pa_part<DT, D, FP>(p, item, false, lds);
+      return;
+    }
   }
+  if constexpr (FS >= 0) pa_part<DT, D, FS>(p, item - (FP >= 0 ? p.items_p : 0), true, lds);
 }
 
-// Joins the parts: D / 4 lanes per row of the output.  The workgroups behind those of the rows
-// add each cached key's weight: w_out = w_in + sum over its columns of 2^(score - log2 total).
+// A wave's view of a row's parts: the log2-scaled maximum and the sum over all of them (-inf
+// and 0 for a row that saw nothing), and this lane's factors 2^(m_s - m) for slots lane and
+// 64 + lane (0 for a part that saw nothing).
+struct PaTotal {
+  float m, l, f0, f1;
+};
+constexpr int PA_MAX_SLOTS = 128;
+
+__device__ __forceinline__ PaTotal pa_total(const PrefixAttnParams& p, int64_t row, int lane) {
+  const int slots = p.np + p.ns;
+  const float2* ml = p.part_ml + row * slots;
+  const float2 none = make_float2(PA_NONE, 0.0f);
+  const float2 a = lane < slots ? ml[lane] : none, b = lane + 64 < slots ? ml[lane + 64] : none;
+  PaTotal r;
+  r.m = fmaxf(a.x, b.x);
+  for (int o = 32; o; o >>= 1) r.m = fmaxf(r.m, __shfl_xor(r.m, o));
+  r.f0 = a.x == PA_NONE ? 0.0f : __builtin_amdgcn_exp2f(a.x - r.m);
+  r.f1 = b.x == PA_NONE ? 0.0f : __builtin_amdgcn_exp2f(b.x - r.m);
+  r.l = a.y * r.f0 + b.y * r.f1;
+  for (int o = 32; o; o >>= 1) r.l += __shfl_xor(r.l, o);
+  return r;
+}
+
+// Joins the parts: a wave per row of the output, D / 4 lanes on a part, 64 / (D / 4) parts at
+// once.  The workgroups behind those of the rows add each cached key's weight:
+// w_out = w_in + sum over its columns of 2^(score - log2 total).
+constexpr int PA_JOIN_KEYS = 4 * PA_NT;
+
 template <int DT, int D>
 __global__ void __launch_bounds__(PA_NT) prefix_join_kernel(PrefixAttnParams p, int row_blocks) {
-  constexpr int LPR = D / 4, RPB = PA_NT / LPR;
-  const int64_t rows = (int64_t)p.B * p.n * p.Hq;
+  constexpr int LPR = D / 4, NG = 64 / LPR;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   if ((int)blockIdx.x < row_blocks) {
-    const int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / LPR;
-    if (row >= rows) return;
-    const int d = (threadIdx.x % LPR) * 4;
-    float m, l;
-    pa_total(p, row, rows, m, l);
+    const int64_t row = (int64_t)blockIdx.x * 4 + wave;
+    if (row >= (int64_t)p.B * p.n * p.Hq) return;
+    const int slots = p.np + p.ns, grp = lane / LPR, d = (lane % LPR) * 4;
+    const PaTotal t = pa_total(p, row, lane);
+    const float* po = p.part_o + row * slots * D + d;
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    if (m != PA_NONE)
-      for (int s = 0; s < p.np + p.ns; ++s) {
-        const float ms = p.part_ml[s * rows + row].x;
-        if (ms == PA_NONE) continue;
-        o += *(const f32x4*)(p.part_o + (s * rows + row) * D + d) *
-             __builtin_amdgcn_exp2f(ms - m);
+    // Four loads in flight a lane.  A part that saw nothing has factor 0 and was not written.
+    for (int s0 = 0; s0 < slots; s0 += 4 * NG) {
+      float f[4];
+      f32x4 v[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int s = s0 + u * NG;
+        f[u] = __shfl(s < 64 ? t.f0 : t.f1, (s & 63) + grp);
+        if (s >= PA_MAX_SLOTS) f[u] = 0.0f;
+        v[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (f[u] != 0.0f) v[u] = *(const f32x4*)(po + (int64_t)(s + grp) * D);
       }
-    if (m != PA_NONE) o *= 1.0f / l;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) o += v[u] * f[u];
+    }
+#pragma unroll
+    for (int x = LPR; x < 64; x <<= 1)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] += __shfl_xor(o[e], x);
+    if (grp) return;
+    if (t.m != PA_NONE) o *= 1.0f / t.l;
     *(uint2*)(p.out + row * D + d) = make_uint2(pack2<DT>(o[0], o[1]), pack2<DT>(o[2], o[3]));
     if (p.lse && d == 0)
-      p.lse[row] = m == PA_NONE ? PA_NONE : (m + log2f(l)) * 0.69314718055994531f;
+      p.lse[row] = t.m == PA_NONE ? PA_NONE : (t.m + log2f(t.l)) * 0.69314718055994531f;
     return;
   }
-  // A workgroup takes PA_NT keys of one (sequence, key/value head).
+  // A workgroup takes PA_JOIN_KEYS keys of one (sequence, key/value head).
   __shared__ float s_total[64];
-  const int chunks = (p.S + PA_NT - 1) / PA_NT;
+  const int chunks = (p.S + PA_JOIN_KEYS - 1) / PA_JOIN_KEYS;
   int it = (int)blockIdx.x - row_blocks;
   const int chunk = it % chunks;
   it /= chunks;
   const int hk = it % p.Hkv, b = it / p.Hkv;
   const int cols = p.n * p.G;
-  for (int c = threadIdx.x; c < cols; c += PA_NT) {
-    float m, l;
-    pa_total(p, ((int64_t)b * p.n + c / p.G) * p.Hq + hk * p.G + c % p.G, rows, m, l);
-    s_total[c] = m == PA_NONE ? INFINITY : m + log2f(l);  // 2^(x - inf) = 0
+  for (int c = wave; c < cols; c += 4) {
+    const PaTotal t =
+        pa_total(p, ((int64_t)b * p.n + c / p.G) * p.Hq + hk * p.G + c % p.G, lane);
+    if (lane == 0) s_total[c] = t.m == PA_NONE ? INFINITY : t.m + log2f(t.l);  // 2^-inf = 0
   }
   __syncthreads();
-  const int key = chunk * PA_NT + threadIdx.x;
-  if (key >= p.S) return;
-  const int64_t at = ((int64_t)b * p.Hkv + hk) * p.S + key;
-  float w = p.w_in ? p.w_in[at] : 0.0f;
-  // Only the columns that see the key: their scores alone were written.
-  const float* sc = p.score + (((int64_t)b * p.Hkv + hk) * cols) * p.spad + key;
   const int row0 = pa_len(p, b) - p.n;
-  float sum = 0.0f;
-  for (int c = 0; c < cols; ++c) {
-    const int at_q = row0 + c / p.G;
-    if (at_q >= key && (!p.window || at_q - key < p.window))
-      sum += __builtin_amdgcn_exp2f(sc[(int64_t)c * p.spad] - s_total[c]);
+  const int64_t head = (int64_t)b * p.Hkv + hk;
+#pragma unroll
+  for (int u = 0; u < PA_JOIN_KEYS / PA_NT; ++u) {
+    const int key = chunk * PA_JOIN_KEYS + u * PA_NT + threadIdx.x;
+    if (key >= p.S) return;
+    // Only the columns that see the key: their scores alone were written.
+    const float* sc = p.score + head * cols * p.spad + key;
+    float sum = 0.0f;
+    for (int c = 0; c < cols; ++c) {
+      const int at = row0 + c / p.G;
+      if (at >= key && (!p.window || at - key < p.window))
+        sum += __builtin_amdgcn_exp2f(sc[(int64_t)c * p.spad] - s_total[c]);
+    }
+    p.w_out[head * p.S + key] = (p.w_in ? p.w_in[head * p.S + key] : 0.0f) + sum;
   }
-  p.w_out[at] = w + sum;
 }
 
 // ---- host -------------------------------------------------------------------------------
 
 struct PrefixPlan {
-  int form_p, form_s;          // -1: no such parts
-  int np, ns, rbp, rbs, spad;
+  int form_p, form_s;  // -1: no such parts
+  int np, ns, chunk_p, chunk_s, rbp, rbs, spad;
   int64_t items_p, items_s, rows;
   size_t off_ml, off_score, bytes;
 };
 
-static int pa_form(int64_t cols) { return cols <= 16 ? 0 : cols <= 32 ? 1 : cols <= 64 ? 2 : 3; }
+// The narrowest form that takes the columns in one block; past 128 the widest one (192 columns
+// at head dim 64, 128 at 128, whose accumulators take the registers).
+static int pa_form(int64_t cols, int D) {
+  for (int f = 0; f < 4; ++f)
+    if (cols <= PA_WIDTH[f]) return f;
+  return D == 64 ? 4 : 3;
+}
 
 static PrefixPlan pa_plan(const nsmoe_prefix_attn_args* a) {
   PrefixPlan pl{};
   const int64_t G = a->n_heads / a->n_kv_heads, B = a->batch, n = a->n_new;
-  const int64_t cus = device_cus();
+  const int64_t slots = 2 * device_cus();  // workgroups that run at once
   pl.rows = B * n * a->n_heads;
-  pl.form_p = a->prefix_len > 0 ? pa_form(B * n * G) : -1;
-  pl.form_s = a->cap > 0 ? pa_form(n * G) : -1;
-  auto splits = [&](int64_t groups, int64_t keys) {
-    // Two workgroups per CU over the launch; a part keeps at least two turns of the few
-    // form's waves, or four tiles of the many form's.
-    const int64_t least = 256;
-    int64_t s = cdiv(2 * cus, groups), most = cdiv(keys, least);
-    s = s < most ? s : most;
-    return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
+  pl.form_p = a->prefix_len > 0 ? pa_form(B * n * G, a->head_dim) : -1;
+  pl.form_s = a->cap > 0 ? pa_form(n * G, a->head_dim) : -1;
+  // Keys per part, whole tiles of all four waves: as few as give `per` parts for each slot,
+  // at least 128 (a tile a wave), and at most 64 parts.
+  auto chunk_of = [&](int64_t groups, int64_t keys, int64_t want) {
+    int64_t parts = want / groups;
+    parts = parts < 1 ? 1 : parts > 64 ? 64 : parts;
+    int64_t c = cdiv(cdiv(keys, parts), 128) * 128;
+    return (int)c;
   };
   if (pl.form_p >= 0) {
     pl.rbp = (int)cdiv(B * n * G, PA_WIDTH[pl.form_p]);
-    pl.np = splits((int64_t)pl.rbp * a->n_kv_heads, a->prefix_len);
-    pl.items_p = (int64_t)pl.np * pl.rbp * a->n_kv_heads;
+    const int64_t groups = (int64_t)pl.rbp * a->n_kv_heads;
+    pl.chunk_p = chunk_of(groups, a->prefix_len, pl.form_p < 2 ? 4 * slots : slots);
+    pl.np = (int)cdiv(a->prefix_len, pl.chunk_p);
+    pl.items_p = pl.np * groups;
   }
   if (pl.form_s >= 0) {
     pl.rbs = (int)cdiv(n * G, PA_WIDTH[pl.form_s]);
-    pl.ns = splits(B * pl.rbs * a->n_kv_heads, a->cap);
-    pl.items_s = (int64_t)pl.ns * pl.rbs * a->n_kv_heads * B;
+    const int64_t groups = B * pl.rbs * a->n_kv_heads;
+    pl.chunk_s = chunk_of(groups, a->cap, 4 * slots);
+    pl.ns = (int)cdiv(a->cap, pl.chunk_s);
+    pl.items_s = pl.ns * groups;
   }
   pl.spad = (int)(cdiv(a->cap, 64) * 64);
-  const size_t slots = (size_t)(pl.np + pl.ns), rows = (size_t)pl.rows;
+  const size_t parts = (size_t)(pl.np + pl.ns), rows = (size_t)pl.rows;
   auto up = [](size_t x) { return (x + 255) / 256 * 256; };
-  pl.off_ml = up(slots * rows * a->head_dim * 4);
-  pl.off_score = pl.off_ml + up(slots * rows * 8);
+  pl.off_ml = up(parts * rows * a->head_dim * 4);
+  pl.off_score = pl.off_ml + up(parts * rows * 8);
   pl.bytes = pl.off_score;
   if (a->weights_out) pl.bytes += up((size_t)B * a->n_kv_heads * n * G * pl.spad * 4);
   return pl;
 }
 
-template <int DT, int D, int FORM>
-static int pa_part_form(const PrefixAttnParams& P, int64_t items, bool own, hipStream_t s) {
-  constexpr int lds = FORM < 2 ? PaGeo<D>::FEW_LDS : PaGeo<D>::MANY_LDS;
-  static_assert(FORM >= 2 || 4 * 16 * (FORM + 1) * (D * 4 + 8) <= lds, "the join fits the ring");
-  prefix_part_kernel<DT, D, FORM><<<(unsigned)items, PA_NT, lds, s>>>(P, own);
+template <int DT, int D, int FP, int FS>
+static int pa_run(const PrefixAttnParams& P, int64_t items, const char* name, hipStream_t s) {
+  constexpr int few = PaGeo<D>::FEW_LDS, many = PaGeo<D>::MANY_LDS;
+  constexpr int lds = (FP >= 2 || FS >= 2) && many > few ? many
+                      : (FP >= 0 && FP < 2) || (FS >= 0 && FS < 2) ? few : many;
+  static_assert(2 * 64 <= PA_MAX_SLOTS, "a lane holds two slots");
+  static_assert(4 * 16 * (D * 4 + 8) <= few, "the join of the waves fits their buffers");
+  NSMOE_REQUIRE(items < INT32_MAX, "prefix_attention: grid too large");
+  KernelTimer timer(name, s);
+  prefix_part_kernel<DT, D, FP, FS><<<(unsigned)items, PA_NT, lds, s>>>(P);
+  timer.stop();
   return check_launch("prefix_part_kernel");
 }
 
-template <int DT, int D>
-static int pa_parts(const PrefixAttnParams& P, int form, int64_t items, bool own, hipStream_t s) {
+// Calls f with the form as a constant.
+template <int D, class F>
+static int pa_with_form(int form, F&& f) {
   switch (form) {
-    case 0: return pa_part_form<DT, D, 0>(P, items, own, s);
-    case 1: return pa_part_form<DT, D, 1>(P, items, own, s);
-    case 2: return pa_part_form<DT, D, 2>(P, items, own, s);
-    default: return pa_part_form<DT, D, 3>(P, items, own, s);
+    case 0: return f(std::integral_constant<int, 0>{});
+    case 1: return f(std::integral_constant<int, 1>{});
+    case 2: return f(std::integral_constant<int, 2>{});
+    case 3: return f(std::integral_constant<int, 3>{});
+    default:
+      if constexpr (D == 64) return f(std::integral_constant<int, 4>{});
+      else return f(std::integral_constant<int, 3>{});
   }
 }
 
 template <int DT, int D>
 static int pa_launch(const PrefixAttnParams& P, const PrefixPlan& pl, hipStream_t s) {
-  if (pl.form_p >= 0) {
-    KernelTimer timer("prefix_part", s);
-    NSMOE_TRY((pa_parts<DT, D>(P, pl.form_p, pl.items_p, false, s)));
-    timer.stop();
+  // Own caches under few columns (a decode step) share the prefix's launch; under many they
+  // are a launch of their own.
+  if (pl.form_p >= 0 && pl.form_s >= 0 && pl.form_s < 2) {
+    const int64_t items = pl.items_p + pl.items_s;
+    NSMOE_TRY(pa_with_form<D>(pl.form_p, [&](auto fp) {
+      constexpr int FP = decltype(fp)::value;
+      return pl.form_s == 0 ? pa_run<DT, D, FP, 0>(P, items, "prefix_part", s)
+                            : pa_run<DT, D, FP, 1>(P, items, "prefix_part", s);
+    }));
+  } else {
+    if (pl.form_p >= 0)
+      NSMOE_TRY(pa_with_form<D>(pl.form_p, [&](auto fp) {
+        return pa_run<DT, D, decltype(fp)::value, -1>(P, pl.items_p, "prefix_part", s);
+      }));
+    if (pl.form_s >= 0)
+      NSMOE_TRY(pa_with_form<D>(pl.form_s, [&](auto fs) {
+        return pa_run<DT, D, -1, decltype(fs)::value>(P, pl.items_s, "own_part", s);
+      }));
   }
-  if (pl.form_s >= 0) {
-    KernelTimer timer("own_part", s);
-    NSMOE_TRY((pa_parts<DT, D>(P, pl.form_s, pl.items_s, true, s)));
-    timer.stop();
-  }
-  const int64_t row_blocks = cdiv(pl.rows, PA_NT / (D / 4));
+  const int64_t row_blocks = cdiv(pl.rows, 4);
   int64_t grid = row_blocks;
-  if (P.w_out) grid += (int64_t)P.B * P.Hkv * cdiv(P.S, PA_NT);
+  if (P.w_out) grid += (int64_t)P.B * P.Hkv * cdiv(P.S, PA_JOIN_KEYS);
   NSMOE_REQUIRE(grid < INT32_MAX, "prefix_attention: grid too large");
   KernelTimer timer("prefix_join", s);
   prefix_join_kernel<DT, D><<<(unsigned)grid, PA_NT, 0, s>>>(P, (int)row_blocks);
@@ -813,8 +919,11 @@ extern "C" int nsmoe_prefix_attention(const nsmoe_prefix_attn_args* a, void* wor
   P.spad = pl.spad;
   P.np = pl.np;
   P.ns = pl.ns;
+  P.chunk_p = pl.chunk_p;
+  P.chunk_s = pl.chunk_s;
   P.rbp = pl.rbp;
   P.rbs = pl.rbs;
+  P.items_p = (int)pl.items_p;
   P.scale_log2 = a->scale * 1.4426950408889634f;
   hipStream_t s = (hipStream_t)stream;
   if (a->head_dim == 64)
