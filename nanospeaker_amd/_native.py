@@ -8,6 +8,7 @@ moe_kernel.py goes through it.
 from __future__ import annotations
 
 import ctypes
+import struct
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libnsmoe.so"
@@ -116,6 +117,22 @@ class BlockNorm(ctypes.Structure):
     _fields_ = [("weight", _vp), ("grad_weight", _vp), ("eps", ctypes.c_float),
                 ("reserved", _i32)]
 
+
+def packer(cls):
+    """A function of the fields of an argument struct in order (arrays element by element,
+    pointers as integers, 0 for NULL) that makes one: one pack of all of them instead of an
+    assignment each (0.6 against 2 to 3 us a call)."""
+    code = {_i32: "i", ctypes.c_float: "f", _i64: "q", _vp: "P"}
+    layout = struct.Struct("@" + "".join(
+        f"{t._length_}{code[t._type_]}" if hasattr(t, "_length_") else code[t]
+        for _, t in cls._fields_))
+    assert layout.size == ctypes.sizeof(cls)
+    pack, make = layout.pack, cls.from_buffer_copy
+    return lambda *values: make(pack(*values))
+
+
+rope_args, logits_args, evict_args, prefix_attn_args = (
+    packer(c) for c in (RopeArgs, LogitsArgs, EvictArgs, PrefixAttnArgs))
 
 SIGNATURES = {
     "nsmoe_last_error": (ctypes.c_char_p, []),

@@ -18,33 +18,44 @@ import torch
 from torch import Tensor
 
 from . import _native as nat
-from .moe_kernel import _stream, _ws, on_device
+from .moe_kernel import _stream, on_device
+from .rope import _writable
 
 _DT16 = {torch.bfloat16: nat.BF16, torch.float16: nat.F16}
 
 
-def _need(ok: bool, what: str) -> None:
-    if not ok:
-        raise ValueError(what)
+def _fail(op: str, what: str):
+    raise ValueError(f"{op}: {what}")
 
 
 def _lens(op: str, lens: Tensor, b: int, device) -> None:
-    _need(lens.dtype == torch.int32 and lens.shape == (b,) and lens.device == device
-          and lens.is_contiguous(),
-          f"{op}: lens must be a contiguous int32 [{b}] on {device}, got {lens.dtype} "
-          f"{tuple(lens.shape)} on {lens.device}")
-
-
-def _wide(t: Tensor) -> bool:
-    """Whether a 16-bit tensor's rows can be read 16 bytes at a time: a contiguous last dim,
-    every other stride and the address a multiple of 16 bytes."""
-    return (t.stride(-1) == 1 and t.data_ptr() % 16 == 0
-            and all(s % 8 == 0 for s, n in zip(t.stride()[:-1], t.shape) if n > 1))
+    if (lens.dtype is not torch.int32 or lens.shape != (b,) or lens.device != device
+            or not lens.is_contiguous()):
+        _fail(op, f"lens must be a contiguous int32 [{b}] on {device}, got {lens.dtype} "
+                  f"{tuple(lens.shape)} on {lens.device}")
 
 
 def _strides(t: Tensor) -> "tuple[int, ...]":
     """The strides before the last dim, 0 where a dim has one element (any stride fits it)."""
     return tuple(s if n > 1 else 0 for s, n in zip(t.stride()[:-1], t.shape))
+
+
+def _rows16(t: Tensor) -> "Optional[tuple[int, ...]]":
+    """The strides before the last dim of a 16-bit tensor whose rows can be read 16 bytes at a
+    time (a contiguous last dim, every other stride and the address a multiple of 16 bytes);
+    None of one whose rows cannot."""
+    s = t.stride()[:-1]
+    bits = 0
+    for x in s:
+        bits |= x
+    if bits & 7:  # a stride of a dim of one element may be anything
+        s = _strides(t)
+        bits = 0
+        for x in s:
+            bits |= x
+    if t.numel() == 0:
+        return s
+    return None if bits & 7 or t.stride(-1) != 1 or t.data_ptr() & 15 else s
 
 
 def shared_prefix_attention(q: Tensor, k_prefix: Optional[Tensor], v_prefix: Optional[Tensor],
@@ -73,64 +84,69 @@ def shared_prefix_attention(q: Tensor, k_prefix: Optional[Tensor], v_prefix: Opt
     head) with weights.
     """
     op = "shared_prefix_attention"
-    _need(q.dim() == 4 and q.is_cuda and q.dtype in _DT16,
-          f"{op}: q must be a bf16 or fp16 [batch, n, heads, dim] GPU tensor, got {q.dtype} "
-          f"{tuple(q.shape)} on {q.device}")
+    if q.dim() != 4 or not q.is_cuda or q.dtype not in _DT16:
+        _fail(op, "q must be a bf16 or fp16 [batch, n, heads, dim] GPU tensor, got "
+                  f"{q.dtype} {tuple(q.shape)} on {q.device}")
     b, n, hq, d = q.shape
-    dev = q.device
-    _need(k.dim() == 4 and k.shape == v.shape and k.shape[0] == b and k.shape[3] == d
-          and k.shape[2] >= 1 and hq % k.shape[2] == 0,
-          f"{op}: k {tuple(k.shape)} and v {tuple(v.shape)} do not go with q {tuple(q.shape)}")
+    dev, dt = q.device, q.dtype
+    if (k.dim() != 4 or k.shape != v.shape or k.shape[0] != b or k.shape[3] != d
+            or k.shape[2] < 1 or hq % k.shape[2]):
+        _fail(op, f"k {tuple(k.shape)} and v {tuple(v.shape)} do not go with q {tuple(q.shape)}")
     s, hk = k.shape[1], k.shape[2]
-    _need((k_prefix is None) == (v_prefix is None), f"{op}: k_prefix without v_prefix")
-    caches = [k, v]
-    p = 0
+    if (k_prefix is None) != (v_prefix is None):
+        _fail(op, "k_prefix without v_prefix, or v_prefix without k_prefix")
+    p = kp = vp = 0
+    skp = svp = (0, 0)
     if k_prefix is not None:
-        _need(k_prefix.dim() == 3 and k_prefix.shape == v_prefix.shape
-              and k_prefix.shape[1:] == (hk, d),
-              f"{op}: prefix {tuple(k_prefix.shape)}, {tuple(v_prefix.shape)}, expected "
-              f"[rows, {hk}, {d}]")
+        if (k_prefix.dim() != 3 or k_prefix.shape != v_prefix.shape or k_prefix.shape[1] != hk
+                or k_prefix.shape[2] != d):
+            _fail(op, f"prefix {tuple(k_prefix.shape)}, {tuple(v_prefix.shape)}, expected [rows, "
+                      f"{hk}, {d}]")
         p = k_prefix.shape[0]
-        caches += [k_prefix, v_prefix]
-    for t in caches:
-        _need(t.dtype == q.dtype and t.device == dev, f"{op}: caches and q differ in type or "
-              "device")
-        _need(t.numel() == 0 or _wide(t), f"{op}: caches need a contiguous last dim, and strides "
-              "and addresses that are multiples of 16 bytes")
+        kp, vp = k_prefix.data_ptr(), v_prefix.data_ptr()
+        skp, svp = _rows16(k_prefix), _rows16(v_prefix)
+    for t in (k, v) if k_prefix is None else (k, v, k_prefix, v_prefix):
+        if t.dtype is not dt or t.device != dev:
+            _fail(op, f"a cache is {t.dtype} on {t.device}, another type or device than q's "
+                      f"{dt} on {dev}")
+    sk, sv = _rows16(k), _rows16(v)
+    if sk is None or sv is None or skp is None or svp is None:
+        _fail(op, "caches need a contiguous last dim, and strides and addresses that are multiples "
+                  "of 16 bytes")
     _lens(op, lens, b, dev)
-    _need(window is None or window >= 1, f"{op}: window {window}")
-    if not _wide(q):
-        q = q.contiguous() if q.data_ptr() % 16 == 0 else q.clone(
-            memory_format=torch.contiguous_format)
-    out = torch.empty((b, n, hq, d), dtype=q.dtype, device=dev)
+    if window is None:
+        window = 0
+    elif window < 1:
+        _fail(op, f"window {window}")
+    sq = _rows16(q)
+    if sq is None:
+        q = q.clone(memory_format=torch.contiguous_format)
+        sq = q.stride()[:-1]
+    out = q.new_empty((b, n, hq, d))
     lse = torch.empty((b, n, hq), dtype=torch.float32, device=dev) if return_lse else None
     if weights is not None or weights_out is not None:
         for name, t in (("weights", weights), ("weights_out", weights_out)):
-            _need(t is None or (t.dtype == torch.float32 and t.shape == (b, hk, s)
-                                and t.device == dev and t.is_contiguous()),
-                  f"{op}: {name} must be a contiguous fp32 {(b, hk, s)} on {dev}")
-        _need(n * (hq // hk) <= 64, f"{op}: weights for at most 64 queries per key head, got "
-              f"{n * (hq // hk)}")
+            if t is not None and (t.dtype is not torch.float32 or t.shape != (b, hk, s)
+                                  or t.device != dev or not t.is_contiguous()):
+                _fail(op, f"{name} must be a contiguous fp32 {(b, hk, s)} on {dev}")
+        if n * (hq // hk) > 64:
+            _fail(op, f"weights for at most 64 queries per key head, got {n * (hq // hk)}")
         if weights_out is None:
             weights_out = torch.empty_like(weights)
-    a = nat.PrefixAttnArgs(
-        dtype=_DT16[q.dtype], head_dim=d, n_heads=hq, n_kv_heads=hk, batch=b, n_new=n,
-        prefix_len=p, cap=s, window=0 if window is None else min(int(window), (1 << 30) - 1),
-        scale=1.0 / math.sqrt(d) if scale is None else float(scale),
-        q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), q_stride=_strides(q),
-        k_stride=_strides(k), v_stride=_strides(v), lens=lens.data_ptr(), out=out.data_ptr(),
-        lse=None if lse is None else lse.data_ptr(),
-        weights=None if weights is None else weights.data_ptr(),
-        weights_out=None if weights_out is None else weights_out.data_ptr())
-    if p:
-        a.k_prefix, a.v_prefix = k_prefix.data_ptr(), v_prefix.data_ptr()
-        a.kp_stride, a.vp_stride = _strides(k_prefix), _strides(v_prefix)
     if b and n:
+        a = nat.prefix_attn_args(
+            _DT16[dt], d, hq, hk, b, n, p, s, min(int(window), (1 << 30) - 1),
+            1.0 / math.sqrt(d) if scale is None else float(scale), q.data_ptr(), kp, vp,
+            k.data_ptr(), v.data_ptr(), *sq, *skp, *svp, *sk, *sv, lens.data_ptr(),
+            out.data_ptr(), 0 if lse is None else lse.data_ptr(),
+            0 if weights is None else weights.data_ptr(),
+            0 if weights_out is None else weights_out.data_ptr())
         lib = nat.lib()
         with on_device(dev):
-            ws = _ws(lib.nsmoe_prefix_attention_workspace_size(a), dev)
-            nat.check(lib.nsmoe_prefix_attention(a, ws.data_ptr(), ws.numel(),
-                                                 _stream(dev.index)), "nsmoe_prefix_attention")
+            size = lib.nsmoe_prefix_attention_workspace_size(a)
+            ws = torch.empty(size, dtype=torch.uint8, device=dev)
+            nat.check(lib.nsmoe_prefix_attention(a, ws.data_ptr(), size, _stream(dev.index)),
+                      "nsmoe_prefix_attention")
     elif weights_out is not None and weights_out is not weights:
         weights_out.zero_() if weights is None else weights_out.copy_(weights)
     if lse is None and weights_out is None:
@@ -154,50 +170,50 @@ def cache_evict(k: Tensor, v: Tensor, weights: Tensor, lens: Tensor, budget: int
     Any 2- or 4-byte type and strides with a contiguous last dim.
     """
     op = "cache_evict"
-    _need(k.dim() == 4 and k.is_cuda and k.element_size() in (2, 4) and k.shape == v.shape
-          and v.dtype == k.dtype and v.device == k.device,
-          f"{op}: k and v must be [batch, rows, heads, dim] GPU tensors of one 2- or 4-byte type, "
-          f"got {k.dtype} {tuple(k.shape)} and {v.dtype} {tuple(v.shape)} on {k.device}")
+    if (k.dim() != 4 or not k.is_cuda or k.element_size() not in (2, 4) or k.shape != v.shape
+            or v.dtype is not k.dtype or v.device != k.device):
+        _fail(op, "k and v must be [batch, rows, heads, dim] GPU tensors of one 2- or 4-byte type, "
+                  f"got {k.dtype} {tuple(k.shape)} and {v.dtype} {tuple(v.shape)} on {k.device}")
     b, s, hk, d = k.shape
     dev = k.device
     budget, recent, sinks = int(budget), int(recent), int(sinks)
-    _need(budget >= 1 and recent >= 0 and sinks >= 0 and recent + sinks <= budget,
-          f"{op}: budget {budget} with {sinks} sinks and {recent} recent rows")
-    _need(weights.shape == (b, hk, s) and weights.dtype == torch.float32 and weights.device == dev,
-          f"{op}: weights must be fp32 {(b, hk, s)} on {dev}, got {weights.dtype} "
-          f"{tuple(weights.shape)} on {weights.device}")
+    if budget < 1 or recent < 0 or sinks < 0 or recent + sinks > budget:
+        _fail(op, f"budget {budget} with {sinks} sinks and {recent} recent rows")
+    if weights.shape != (b, hk, s) or weights.dtype is not torch.float32 or weights.device != dev:
+        _fail(op, f"weights must be fp32 {(b, hk, s)} on {dev}, got {weights.dtype} "
+                  f"{tuple(weights.shape)} on {weights.device}")
     _lens(op, lens, b, dev)
+    rows = budget
     if out is None:
-        k_out = torch.empty((b, budget, hk, d), dtype=k.dtype, device=dev)
+        k_out = k.new_empty((b, budget, hk, d))
         v_out = torch.empty_like(k_out)
-        w_out = torch.empty((b, hk, budget), dtype=torch.float32, device=dev)
+        w_out = weights.new_empty((b, hk, budget))
     else:
         k_out, v_out, w_out = out
         rows = k_out.shape[1] if k_out.dim() == 4 else -1
-        _need(rows >= budget and k_out.shape == v_out.shape == (b, rows, hk, d)
-              and w_out.shape == (b, hk, rows) and k_out.dtype == v_out.dtype == k.dtype
-              and w_out.dtype == torch.float32
-              and k_out.device == v_out.device == w_out.device == dev,
-              f"{op}: out must be k, v {(b, f'>= {budget}', hk, d)} and weights "
-              f"{(b, hk, f'>= {budget}')} of the inputs' types")
-        for t in out:
-            for i in (k, v, weights):
-                _need(not _share(t, i), f"{op}: out shares memory with the inputs")
+        if (rows < budget or not k_out.shape == v_out.shape == (b, rows, hk, d)
+                or w_out.shape != (b, hk, rows) or not k_out.dtype == v_out.dtype == k.dtype
+                or w_out.dtype is not torch.float32
+                or not k_out.device == v_out.device == w_out.device == dev):
+            _fail(op, f"out must be k, v {(b, f'>= {budget}', hk, d)} and weights "
+                      f"{(b, hk, f'>= {budget}')} of the inputs' types")
+        for i, t in enumerate(out):
+            if any(_share(t, o) for o in (k, v, weights, *out[:i])):
+                _fail(op, "out shares memory with the inputs or with itself")
+            if not _writable(t):
+                _fail(op, "out has elements that share memory")
     for t in (k, v, k_out, v_out, weights, w_out):
-        _need(t.numel() == 0 or t.shape[-1] == 1 or t.stride(-1) == 1,
-              f"{op}: the last dim must be contiguous")
+        if t.stride(-1) != 1 and t.shape[-1] > 1 and t.numel():
+            _fail(op, "the last dim must be contiguous")
     index = torch.empty((b, hk, budget), dtype=torch.int32, device=dev)
     lens_out = torch.empty_like(lens)
     if b and hk and d:
-        a = nat.EvictArgs(
-            elem_bytes=k.element_size(), n_kv_heads=hk, head_dim=d, zero_tail=int(out is None),
-            batch=b, cap=s, out_cap=k_out.shape[1], budget=budget, recent=recent, sinks=sinks,
-            k=k.data_ptr(), v=v.data_ptr(), k_out=k_out.data_ptr(), v_out=v_out.data_ptr(),
-            k_stride=_strides(k), v_stride=_strides(v), k_out_stride=_strides(k_out),
-            v_out_stride=_strides(v_out), weights=weights.data_ptr(),
-            weights_out=w_out.data_ptr(), weights_stride=_strides(weights),
-            weights_out_stride=_strides(w_out), lens=lens.data_ptr(),
-            lens_out=lens_out.data_ptr(), index=index.data_ptr())
+        a = nat.evict_args(
+            k.element_size(), hk, d, out is None, b, s, rows, budget, recent, sinks,
+            k.data_ptr(), v.data_ptr(), k_out.data_ptr(), v_out.data_ptr(), *_strides(k),
+            *_strides(v), *_strides(k_out), *_strides(v_out), weights.data_ptr(),
+            w_out.data_ptr(), *_strides(weights), *_strides(w_out), lens.data_ptr(),
+            lens_out.data_ptr(), index.data_ptr())
         with on_device(dev):
             nat.check(nat.lib().nsmoe_cache_evict(a, _stream(dev.index)), "nsmoe_cache_evict")
     return k_out, v_out, w_out, index, lens_out

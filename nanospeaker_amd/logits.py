@@ -14,10 +14,11 @@ from . import _native as nat
 from .moe_kernel import _DT, _stream, on_device
 
 
-def _vector(name: str, t: Optional[Tensor], n: int, dtype, device) -> Optional[int]:
+def _vector(name: str, t: Optional[Tensor], n: int, dtype, device) -> int:
+    """The address of a [n] operand, 0 for None."""
     if t is None:
-        return None
-    if t.dtype != dtype or t.shape != (n,) or t.device != device or not t.is_contiguous():
+        return 0
+    if t.dtype is not dtype or t.shape != (n,) or t.device != device or not t.is_contiguous():
         raise ValueError(f"penalize_logits: {name} must be a contiguous {dtype} [{n}] on {device}, "
                          f"got {t.dtype} {tuple(t.shape)} on {t.device}")
     return t.data_ptr()
@@ -27,7 +28,7 @@ def _rows(name: str, t: Tensor, b: int, n: int, dtype, device) -> "tuple[int, in
     """(address, row stride) of a [b, n] operand, or of one row [n] or [1, n] for all."""
     if t.dim() == 1:
         t = t.unsqueeze(0)
-    if (t.dtype != dtype or t.dim() != 2 or t.shape[0] not in (1, b) or t.shape[1] != n
+    if (t.dtype is not dtype or t.dim() != 2 or t.shape[0] not in (1, b) or t.shape[1] != n
             or t.device != device or (t.stride(1) != 1 and n > 1)):
         raise ValueError(f"penalize_logits: {name} must be {dtype} [{b}, {n}] or [{n}] on {device} "
                          f"with contiguous rows, got {t.dtype} {tuple(t.shape)} on {t.device}")
@@ -63,7 +64,7 @@ def penalize_logits(logits: Tensor, history: Optional[Tensor] = None,
     if v > 1 and logits.stride(1) != 1:
         raise ValueError("penalize_logits: the rows of logits must be contiguous")
     if out is None:
-        out = torch.empty((b, v), dtype=logits.dtype, device=dev)
+        out = logits.new_empty((b, v))
     elif (out.shape != (b, v) or out.device != dev or out.dtype not in (logits.dtype, torch.float32)
           or (v > 1 and out.stride(1) != 1) or (b > 1 and out.stride(0) < v)):
         raise ValueError(f"penalize_logits: out must be [{b}, {v}] with contiguous rows of the "
@@ -72,7 +73,7 @@ def penalize_logits(logits: Tensor, history: Optional[Tensor] = None,
             out.data_ptr() == logits.data_ptr() and out.dtype == logits.dtype
             and (b == 1 or out.stride(0) == logits.stride(0))):
         raise ValueError("penalize_logits: out overlaps logits without being them")
-    f = {}
+    n = hist = hist_s = 0
     if history is None:
         if any(t is not None for t in (repetition, frequency, presence, lens, prompt_lens)):
             raise ValueError("penalize_logits: penalties and lengths need a history")
@@ -82,21 +83,16 @@ def penalize_logits(logits: Tensor, history: Optional[Tensor] = None,
         n = history.shape[1]
         if history.shape[0] != b:
             raise ValueError(f"penalize_logits: history of {history.shape[0]} rows for {b}")
-        p, s = _rows("history", history, b, n, torch.int64, dev)
-        f.update(history=p if n else None, history_stride=s, history_cap=n)
-    f32 = torch.float32
-    f.update(lens=_vector("lens", lens, b, torch.int32, dev),
-             prompt_lens=_vector("prompt_lens", prompt_lens, b, torch.int32, dev),
-             repetition=_vector("repetition", repetition, b, f32, dev),
-             frequency=_vector("frequency", frequency, b, f32, dev),
-             presence=_vector("presence", presence, b, f32, dev))
-    if bias is not None:
-        f["bias"], f["bias_stride"] = _rows("bias", bias, b, v, f32, dev)
-    if mask is not None:
-        f["mask"], f["mask_stride"] = _rows("mask", mask, b, (v + 31) // 32, torch.int32, dev)
-    a = nat.LogitsArgs(dtype=_DT[logits.dtype], out_dtype=_DT[out.dtype], batch=b, vocab=v,
-                       logits=logits.data_ptr(), out=out.data_ptr(),
-                       logits_stride=logits.stride(0), out_stride=out.stride(0), **f)
+        hist, hist_s = _rows("history", history, b, n, torch.int64, dev)
+    i32, f32 = torch.int32, torch.float32
+    a = nat.logits_args(
+        _DT[logits.dtype], _DT[out.dtype], b, v, 0, logits.data_ptr(), out.data_ptr(),
+        logits.stride(0), out.stride(0), hist, hist_s, n, _vector("lens", lens, b, i32, dev),
+        _vector("prompt_lens", prompt_lens, b, i32, dev),
+        _vector("repetition", repetition, b, f32, dev),
+        _vector("frequency", frequency, b, f32, dev), _vector("presence", presence, b, f32, dev),
+        *((0, 0) if bias is None else _rows("bias", bias, b, v, f32, dev)),
+        *((0, 0) if mask is None else _rows("mask", mask, b, (v + 31) // 32, i32, dev)))
     with on_device(dev):
         nat.check(nat.lib().nsmoe_penalize_logits(a, _stream(dev.index)), "nsmoe_penalize_logits")
     return out

@@ -81,45 +81,36 @@ def _writable(t: Tensor) -> bool:
     return True
 
 
-def _heads(name: str, t: Tensor) -> Tensor:
-    """t as [batch, tokens, heads, dim] with a contiguous last dim."""
-    if t.dim() == 3:
-        t = t.unsqueeze(0)
-    if t.dim() != 4:
-        raise ValueError(f"rotary_embed: {name} {tuple(t.shape)}, expected [batch, tokens, heads, "
-                         "dim] or [tokens, heads, dim]")
-    if not t.is_cuda or t.dtype not in _DT:
-        raise ValueError(f"rotary_embed: {name} must be a bf16, fp16 or fp32 GPU tensor, got "
-                         f"{t.dtype} on {t.device}")
-    return t
+_NO_STRIDES = (0, 0, 0)
 
 
 def _launch(q: Optional[Tensor], k: Optional[Tensor], positions: Tensor, freqs: Tensor,
             interleaved: bool, amplitude: float, inverse: bool, inplace: bool):
     """The kernel over 4-d q and k (either may be None): their rotations."""
-    some = q if q is not None else k
-    outs, fields, keep = [], {}, []
-    for name, t in (("q", q), ("k", k)):
-        if t is None:
-            outs.append(None)
-            continue
-        if t.stride(3) != 1 and t.shape[3] > 1:
-            t = t.contiguous()
-        o = t if inplace else torch.empty(t.shape, dtype=t.dtype, device=t.device)
-        outs.append(o)
-        fields[name], fields[name + "_out"] = t.data_ptr(), o.data_ptr()
-        fields["n_" + name] = t.shape[2]
-        fields[name + "_stride"] = t.stride()[:3]
-        fields[name + "_out_stride"] = o.stride()[:3]
-        keep.append(t)  # a copy lives until it is read
+    some = k if q is None else q
+    dev = some.device
     b, n, _, d = some.shape
-    a = nat.RopeArgs(dtype=_DT[some.dtype], interleaved=int(interleaved), inverse=int(inverse),
-                     amplitude=amplitude, batch=b, n_tokens=n, head_dim=d,
-                     rot_dim=2 * freqs.numel(), positions=positions.data_ptr(),
-                     pos_stride=positions.stride(), freqs=freqs.data_ptr(), **fields)
-    with on_device(some.device):
-        nat.check(nat.lib().nsmoe_rope(a, _stream(some.device.index)), "nsmoe_rope")
-    return outs
+    hq = hk = qp = kp = op = okp = 0
+    sq = sk = soq = sok = _NO_STRIDES
+    oq = ok = None
+    if q is not None:
+        if q.stride(3) != 1 and d > 1:
+            q = q.contiguous()
+        oq = q if inplace else q.new_empty(q.shape)
+        hq, qp, op = q.shape[2], q.data_ptr(), oq.data_ptr()
+        sq, soq = q.stride()[:3], oq.stride()[:3]
+    if k is not None:
+        if k.stride(3) != 1 and d > 1:
+            k = k.contiguous()
+        ok = k if inplace else k.new_empty(k.shape)
+        hk, kp, okp = k.shape[2], k.data_ptr(), ok.data_ptr()
+        sk, sok = k.stride()[:3], ok.stride()[:3]
+    a = nat.rope_args(_DT[some.dtype], interleaved, inverse, amplitude, b, n, hq, hk, d,
+                      2 * freqs.shape[0], qp, kp, op, okp, *sq, *sk, *soq, *sok,
+                      positions.data_ptr(), *positions.stride(), freqs.data_ptr())
+    with on_device(dev):
+        nat.check(nat.lib().nsmoe_rope(a, _stream(dev.index)), "nsmoe_rope")
+    return oq, ok
 
 
 class _Rotate(torch.autograd.Function):
@@ -130,7 +121,7 @@ class _Rotate(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(positions, freqs)
         ctx.how = (interleaved, amplitude, inverse)
-        return tuple(_launch(q, k, positions, freqs, interleaved, amplitude, inverse, False))
+        return _launch(q, k, positions, freqs, interleaved, amplitude, inverse, False)
 
     @staticmethod
     def backward(ctx, gq, gk):
@@ -156,21 +147,26 @@ def rotary_embed(q: Tensor, k: Optional[Tensor], positions: Tensor, freqs: Tenso
     k.  `inplace` writes into q and k themselves (which must not share elements) and returns
     them; it is for calls that nothing differentiates.
     """
-    flat = q.dim() == 3
-    q4 = _heads("q", q)
-    k4 = None if k is None else _heads("k", k)
-    if k4 is not None and (k4.shape[:2] != q4.shape[:2] or k4.shape[3] != q4.shape[3]
-                           or k4.dtype != q4.dtype or k4.device != q4.device
-                           or k.dim() != q.dim()):
+    if q.dim() not in (3, 4) or not q.is_cuda or q.dtype not in _DT:
+        raise ValueError("rotary_embed: q must be a bf16, fp16 or fp32 [batch, tokens, heads, dim] "
+                         "or [tokens, heads, dim] GPU tensor, got "
+                         f"{q.dtype} {tuple(q.shape)} on {q.device}")
+    if k is not None and (k.dim() != q.dim() or k.shape[:-2] != q.shape[:-2]
+                          or k.shape[-1] != q.shape[-1] or k.dtype != q.dtype
+                          or k.device != q.device):
         raise ValueError(f"rotary_embed: k {tuple(k.shape)} {k.dtype} does not go with q "
                          f"{tuple(q.shape)} {q.dtype}")
+    flat = q.dim() == 3
+    q4, k4 = q, k
+    if flat:
+        q4, k4 = q.unsqueeze(0), None if k is None else k.unsqueeze(0)
     b, n, _, d = q4.shape
-    if positions.dtype != torch.int64 or positions.device != q.device:
+    if positions.dtype is not torch.int64 or positions.device != q.device:
         raise ValueError(f"rotary_embed: positions must be int64 on {q.device}, got "
                          f"{positions.dtype} on {positions.device}")
     if positions.shape != (b, n):
         positions = positions.expand(b, n)
-    if freqs.dtype != torch.float64 or freqs.device != q.device or freqs.dim() != 1 or not (
+    if freqs.dtype is not torch.float64 or freqs.device != q.device or freqs.dim() != 1 or not (
             2 <= 2 * freqs.shape[0] <= d):
         raise ValueError(f"rotary_embed: freqs must be fp64 [rot_dim / 2] on {q.device}, rot_dim "
                          f"2 .. {d}; got {freqs.dtype} {tuple(freqs.shape)} on {freqs.device}")
