@@ -14,7 +14,7 @@
 //
 // A workgroup takes `tok` consecutive tokens: its threads first make the tok x rot / 2 cosines
 // and sines once, into LDS (they are shared by every head of the token), then stream the
-// heads of q and k, VP planes (two VP-element vectors) a thread and step.  Bound by HBM at
+// heads of q and k, VP planes a thread and step in 16-byte vectors.  Bound by HBM at
 // long calls (each element read once and written once) and by launch latency at decode ones.
 #include "../../include/nsmoe.h"
 #include "gemm_core.h"
@@ -33,31 +33,46 @@ struct RopeTensor {
   int64_t db, dt, dh;  // output strides
 };
 
+// Division by a divisor that a whole launch shares: the high half of a product with
+// floor(2^32 / d), which is the quotient or one less, and one correction.
+struct RopeDiv {
+  uint32_t d, mul;
+  __device__ __forceinline__ uint32_t div(uint32_t n) const {
+    const uint32_t q = __umulhi(n, mul);
+    return n - q * d >= d ? q + 1 : q;
+  }
+};
+static RopeDiv rope_div(int64_t d) {
+  return RopeDiv{(uint32_t)d, d == 1 ? 0xffffffffu : (uint32_t)((1ull << 32) / (uint64_t)d)};
+}
+
 struct RopeParams {
   RopeTensor q, k;
   const int64_t* pos;
   int64_t pb, pt;  // position strides in elements
   const double* freq;
   int64_t rows, T;
+  RopeDiv by_half, by_tok, by_head;  // planes; a token's and a head's items
   int nq, nk, D, rot, tok;
-  int copy_tail;  // dims [rot, D) are copied (0: the call is in place)
   float amp, sign;
 };
 
-template <int DT, int N> struct RopeVec {  // N elements as one (or two) vector accesses
+template <int DT, int N> struct RopeVec {
   typename Elem<DT>::T e[N];
 };
 
-template <int DT, int N>
+// N elements as one access: from an address that is a multiple of their size (WIDE), or of one
+// element's.
+template <int DT, int N, bool WIDE>
 __device__ __forceinline__ RopeVec<DT, N> rope_load(const char* p) {
   RopeVec<DT, N> v;
-  constexpr int B = N * (int)sizeof(v.e[0]), A = B < 16 ? B : 16;
+  constexpr int B = N * (int)sizeof(v.e[0]), A = WIDE ? (B < 16 ? B : 16) : (int)sizeof(v.e[0]);
   __builtin_memcpy(&v, __builtin_assume_aligned(p, A), B);
   return v;
 }
-template <int DT, int N>
+template <int DT, int N, bool WIDE>
 __device__ __forceinline__ void rope_store(char* p, const RopeVec<DT, N>& v) {
-  constexpr int B = N * (int)sizeof(v.e[0]), A = B < 16 ? B : 16;
+  constexpr int B = N * (int)sizeof(v.e[0]), A = WIDE ? (B < 16 ? B : 16) : (int)sizeof(v.e[0]);
   __builtin_memcpy(__builtin_assume_aligned(p, A), &v, B);
 }
 
@@ -65,12 +80,20 @@ template <int DT, int VP, bool IL>
 __global__ void __launch_bounds__(RP_NT) rope_kernel(RopeParams p) {
   constexpr int ES = (int)sizeof(typename Elem<DT>::T);
   __shared__ __attribute__((aligned(16))) float s_cos[RP_MAX_TRIG], s_sin[RP_MAX_TRIG];
+  __shared__ int64_t s_at[RP_MAX_TOK][4];  // a token's offsets into q, k and the outputs
   const int half = p.rot / 2;
   const int64_t row0 = (int64_t)blockIdx.x * p.tok;
   const int ntok = (int)min((int64_t)p.tok, p.rows - row0);
-
+  if (threadIdx.x < ntok) {
+    const int64_t row = row0 + threadIdx.x, b = row / p.T, t = row - b * p.T;
+    int64_t* at = s_at[threadIdx.x];
+    at[0] = b * p.q.sb + t * p.q.st;
+    at[1] = b * p.q.db + t * p.q.dt;
+    at[2] = b * p.k.sb + t * p.k.st;
+    at[3] = b * p.k.db + t * p.k.dt;
+  }
   for (int i = threadIdx.x; i < ntok * half; i += RP_NT) {
-    const int t = i / half, j = i - t * half;
+    const int t = (int)p.by_half.div(i), j = i - t * half;
     const int64_t row = row0 + t, b = row / p.T;
     const double pos = (double)p.pos[b * p.pb + (row - b * p.T) * p.pt];
     const double turns = pos * (p.freq[j] * 0.15915494309189533577);  // 1 / (2 pi)
@@ -82,30 +105,31 @@ __global__ void __launch_bounds__(RP_NT) rope_kernel(RopeParams p) {
   }
   __syncthreads();
 
-  // Items of a token: heads x (half / VP rotated vectors pairs, then tail vectors of VP).
+  // Items of a token: heads x (half / VP vectors or pairs of vectors to turn, then the tail's
+  // vectors, as wide as those).
+  constexpr bool WIDE = VP > 1;
+  constexpr int TV = IL && WIDE ? 2 * VP : VP;
   const int nrot = half / VP;
-  const int ntail = p.copy_tail ? (p.D - p.rot) / VP : 0;
-  const int per_head = nrot + ntail, per_tok = (p.nq + p.nk) * per_head;
-  for (int i = threadIdx.x; i < ntok * per_tok; i += RP_NT) {
-    const int t = i / per_tok, u = i - t * per_tok;
-    int h = u / per_head;
-    const int c = u - h * per_head;
-    const int64_t row = row0 + t, b = row / p.T, tt = row - b * p.T;
+  const int n_items = ntok * (int)p.by_tok.d;
+#pragma unroll 2
+  for (int i = threadIdx.x; i < n_items; i += RP_NT) {
+    const int t = (int)p.by_tok.div(i), u = i - t * (int)p.by_tok.d;
+    int h = (int)p.by_head.div(u);
+    const int c = u - h * (int)p.by_head.d;
     const bool is_k = h >= p.nq;
-    const RopeTensor& x = is_k ? p.k : p.q;
     if (is_k) h -= p.nq;
-    const char* src = x.src + b * x.sb + tt * x.st + h * x.sh;
-    char* dst = x.dst + b * x.db + tt * x.dt + h * x.dh;
+    const char* src = is_k ? p.k.src + s_at[t][2] + h * p.k.sh : p.q.src + s_at[t][0] + h * p.q.sh;
+    char* dst = is_k ? p.k.dst + s_at[t][3] + h * p.k.dh : p.q.dst + s_at[t][1] + h * p.q.dh;
     if (c >= nrot) {
-      const int64_t off = (int64_t)(p.rot + (c - nrot) * VP) * ES;
-      rope_store<DT, VP>(dst + off, rope_load<DT, VP>(src + off));
+      const int64_t off = (int64_t)(p.rot + (c - nrot) * TV) * ES;
+      rope_store<DT, TV, WIDE>(dst + off, rope_load<DT, TV, WIDE>(src + off));
       continue;
     }
     const float* cs = s_cos + t * half + c * VP;
     const float* sn = s_sin + t * half + c * VP;
     if constexpr (IL) {
       const int64_t off = (int64_t)c * 2 * VP * ES;
-      RopeVec<DT, 2 * VP> v = rope_load<DT, 2 * VP>(src + off);
+      RopeVec<DT, 2 * VP> v = rope_load<DT, 2 * VP, WIDE>(src + off);
       float o[2 * VP];
 #pragma unroll
       for (int e = 0; e < VP; ++e) {
@@ -114,10 +138,11 @@ __global__ void __launch_bounds__(RP_NT) rope_kernel(RopeParams p) {
         o[2 * e + 1] = bb * cs[e] + a * sn[e];
       }
       round_to<DT>(o, v.e);
-      rope_store<DT, 2 * VP>(dst + off, v);
+      rope_store<DT, 2 * VP, WIDE>(dst + off, v);
     } else {
       const int64_t lo = (int64_t)c * VP * ES, hi = lo + (int64_t)half * ES;
-      RopeVec<DT, VP> va = rope_load<DT, VP>(src + lo), vb = rope_load<DT, VP>(src + hi);
+      RopeVec<DT, VP> va = rope_load<DT, VP, WIDE>(src + lo);
+      RopeVec<DT, VP> vb = rope_load<DT, VP, WIDE>(src + hi);
       float oa[VP], ob[VP];
 #pragma unroll
       for (int e = 0; e < VP; ++e) {
@@ -127,24 +152,27 @@ __global__ void __launch_bounds__(RP_NT) rope_kernel(RopeParams p) {
       }
       round_to<DT>(oa, va.e);
       round_to<DT>(ob, vb.e);
-      rope_store<DT, VP>(dst + lo, va);
-      rope_store<DT, VP>(dst + hi, vb);
+      rope_store<DT, VP, WIDE>(dst + lo, va);
+      rope_store<DT, VP, WIDE>(dst + hi, vb);
     }
   }
 }
 
-template <int DT, int VP>
-static void rope_run(const RopeParams& P, bool il, unsigned grid, hipStream_t s) {
-  if (il) rope_kernel<DT, VP, true><<<grid, RP_NT, 0, s>>>(P);
-  else rope_kernel<DT, VP, false><<<grid, RP_NT, 0, s>>>(P);
+// vp: planes of a thread and step, 16 bytes' worth (8 or 4 elements; half as many pairs) or a
+// half of that, or one.
+template <int DT, bool IL>
+static void rope_run(const RopeParams& P, int vp, unsigned grid, hipStream_t s) {
+  constexpr int W = 16 / (int)sizeof(typename Elem<DT>::T) / (IL ? 2 : 1);
+  if (vp == W) rope_kernel<DT, W, IL><<<grid, RP_NT, 0, s>>>(P);
+  else if (W > 2 && vp == W / 2) rope_kernel<DT, (W > 2 ? W / 2 : 1), IL><<<grid, RP_NT, 0, s>>>(P);
+  else rope_kernel<DT, 1, IL><<<grid, RP_NT, 0, s>>>(P);
 }
 
 template <int DT>
 static int rope_launch(const RopeParams& P, int vp, bool il, unsigned grid, hipStream_t s) {
   KernelTimer timer("rope", s);
-  if (vp == 8) rope_run<DT, 8>(P, il, grid, s);
-  else if (vp == 4) rope_run<DT, 4>(P, il, grid, s);
-  else rope_run<DT, 1>(P, il, grid, s);
+  if (il) rope_run<DT, true>(P, vp, grid, s);
+  else rope_run<DT, false>(P, vp, grid, s);
   timer.stop();
   return check_launch("rope_kernel");
 }
@@ -172,9 +200,8 @@ extern "C" int nsmoe_rope(const nsmoe_rope_args* a, void* stream) {
                 "rope: NULL pointer");
   const int es = a->dtype == DT_F32 ? 4 : 2;
   RopeParams P{};
-  // The widest vectors that the planes, the tail and every address allow: 8 planes a thread
-  // and step (16 bytes of a 16-bit half), 4 where the planes are a multiple of 4 only, else
-  // element by element.
+  // The widest vectors that the planes, the tail and every address allow, up to 16 bytes: the
+  // planes of a thread and step are 16 bytes of each half of a head, or 16 bytes of pairs.
   uint64_t bits = 0;  // of every address and stride, in bytes
   auto take = [&](RopeTensor& t, const void* src, void* dst, const int64_t* si, const int64_t* so) {
     t = RopeTensor{(const char*)src, (char*)dst, si[0] * es, si[1] * es, si[2] * es,
@@ -185,13 +212,19 @@ extern "C" int nsmoe_rope(const nsmoe_rope_args* a, void* stream) {
   if (a->n_q) take(P.q, a->q, a->q_out, a->q_stride, a->q_out_stride);
   if (a->n_k) take(P.k, a->k, a->k_out, a->k_stride, a->k_out_stride);
   NSMOE_REQUIRE((bits & (uint64_t)(es - 1)) == 0, "rope: misaligned pointer");
+  const bool il = a->interleaved != 0;
   const bool in_place = (!a->n_q || a->q == a->q_out) && (!a->n_k || a->k == a->k_out);
   const int half = a->rot_dim / 2, tail = a->head_dim - a->rot_dim;
   auto fits = [&](int vp) {
-    const uint64_t align = (uint64_t)(vp * es < 16 ? vp * es : 16);
-    return half % vp == 0 && (in_place || tail % vp == 0) && (bits & (align - 1)) == 0;
+    const int unit = il ? 2 * vp : vp;  // elements of a vector
+    return half % vp == 0 && (in_place || tail % unit == 0) && (bits & (uint64_t)(unit * es - 1)) == 0;
   };
-  const int vp = fits(8) ? 8 : fits(4) ? 4 : 1;
+  const int widest = 16 / es / (il ? 2 : 1);
+  const int vp = fits(widest) ? widest : widest > 2 && fits(widest / 2) ? widest / 2 : 1;
+  const int per_head = half / vp + (in_place ? 0 : tail / (il && vp > 1 ? 2 * vp : vp));
+  P.by_half = rope_div(half);
+  P.by_head = rope_div(per_head);
+  P.by_tok = rope_div((int64_t)per_head * (a->n_q + a->n_k));
   P.pos = a->positions;
   P.pb = a->pos_stride[0];
   P.pt = a->pos_stride[1];
@@ -202,19 +235,17 @@ extern "C" int nsmoe_rope(const nsmoe_rope_args* a, void* stream) {
   P.nk = a->n_k;
   P.D = a->head_dim;
   P.rot = a->rot_dim;
-  P.copy_tail = !in_place;
   P.amp = a->amplitude;
   P.sign = a->inverse ? -1.0f : 1.0f;
-  // Tokens per workgroup: one while the call has fewer tokens than two workgroups a CU, then
-  // as many as keep that number, at most 16 and what the LDS table holds.
-  int64_t tok = P.rows / (2 * device_cus());
+  // Tokens per workgroup: as many as leave eight workgroups a CU (what fits at once), at most
+  // 16 and what the LDS table holds.
+  int64_t tok = P.rows / (8 * device_cus());
   tok = tok < 1 ? 1 : tok > RP_MAX_TOK ? RP_MAX_TOK : tok;
   if (tok > RP_MAX_TRIG / half) tok = RP_MAX_TRIG / half;
   P.tok = (int)tok;
   const int64_t grid = cdiv(P.rows, tok);
   NSMOE_REQUIRE(grid < INT32_MAX, "rope: grid too large");
   hipStream_t s = (hipStream_t)stream;
-  const bool il = a->interleaved != 0;
   switch (a->dtype) {
     case DT_BF16: return rope_launch<DT_BF16>(P, vp, il, (unsigned)grid, s);
     case DT_F16: return rope_launch<DT_F16>(P, vp, il, (unsigned)grid, s);

@@ -133,9 +133,10 @@ def test_operands_off_the_vector_alignment():
     odd = flat[1:].view(2, 11, 3, 65)[..., :64]
     heads_first = odd.transpose(1, 2).contiguous().transpose(1, 2)
     last = odd.transpose(2, 3).contiguous().transpose(2, 3)  # last dim not contiguous
-    want, slack = ref(odd, pos[None], freqs, False, 1.0)
-    for x in (odd, heads_first, last):
-        check("x", rotary_embed(x, None, pos, freqs)[0], want, slack)
+    for il in (False, True):
+        want, slack = ref(odd, pos[None], freqs, il, 1.0)
+        for x in (odd, heads_first, last):
+            check("x", rotary_embed(x, None, pos, freqs, interleaved=il)[0], want, slack)
     shared = odd[:, :, :1].expand(2, 11, 3, 64)
     y, _ = rotary_embed(shared, None, pos, freqs)
     check("expanded", y, *ref(shared, pos[None], freqs, False, 1.0))
