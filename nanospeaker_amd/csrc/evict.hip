@@ -10,13 +10,14 @@
 //                        and 10 bits in LDS), then one ordered pass that writes the kept
 //                        indices, weights and the new length.  Each wave owns a contiguous
 //                        run of the row, so an index's place is the counts of the waves
-//                        before it plus a ballot within the wave.
+//                        before it plus a ballot within the wave.  Up to 8192 rows the weights
+//                        are read once and stay in registers (8 a lane) over the passes;
+//                        longer rows are read again each pass, from L2.
 //   evict_move_kernel    copies the kept key and value rows, 16 bytes a thread, by those
 //                        indices.
 //
-// The selection reads a row of weights four times, from L2 after the first; the move reads and
-// writes the kept rows once, which is nearly all of the traffic: bound by HBM at large caches,
-// by the selection's chain of passes at small ones.
+// The move reads and writes the kept rows once, which is nearly all of the traffic: bound by
+// HBM at large caches, by the selection's chain of passes at small ones.
 //
 // Weights order as floats with -0 equal to +0; a NaN counts as the largest (it is kept, where
 // it can be seen, rather than lost).
@@ -29,6 +30,7 @@ namespace nsmoe {
 constexpr int EV_NT = 1024;
 constexpr int EV_WAVES = EV_NT / 64;
 constexpr int EV_BINS = 2048;
+constexpr int EV_HOLD = 8;  // weights of a lane in registers
 constexpr int EV_MOVE_NT = 256;
 
 struct EvictParams {
@@ -82,20 +84,44 @@ __global__ void __launch_bounds__(EV_NT) evict_select_kernel(EvictParams p) {
     return;
   }
   const int lo = p.sinks, hi = n - p.recent;  // the rows that compete
+  // The wave's run of [0, n): whole steps of 64, in turns of EV_HOLD steps.
+  const int steps = ((n + EV_WAVES - 1) / EV_WAVES + 63) / 64;
+  const int w0 = wave * steps * 64, w1 = min(n, w0 + steps * 64);
+  const int turns = (steps + EV_HOLD - 1) / EV_HOLD;
+  float f[EV_HOLD];
+  auto load = [&](int turn) {
+#pragma unroll
+    for (int u = 0; u < EV_HOLD; ++u) {
+      const int i = w0 + (turn * EV_HOLD + u) * 64 + lane;
+      f[u] = i < w1 ? w[i] : 0.0f;
+    }
+  };
+  // each(row, weight) over the wave's rows, 64 lanes a step (past the run's end: row >= w1)
+  auto sweep = [&](auto&& each) {
+    for (int turn = 0; turn < turns; ++turn) {
+      if (turns > 1) load(turn);
+#pragma unroll
+      for (int u = 0; u < EV_HOLD; ++u)
+        if (turn * EV_HOLD + u < steps) each(w0 + (turn * EV_HOLD + u) * 64 + lane, f[u]);
+    }
+  };
+  if (turns == 1) load(0);
   uint32_t left = (uint32_t)(m - p.sinks - p.recent);
   // The descent: `prefix` holds the decided high bits of the threshold key, `left` how many
   // keys are still to be taken among those that share it.  left == 0 takes none: any
   // threshold above every key would do, and the top one with no ties taken is such.
   uint32_t prefix = 0, mask = 0;
   const int shift[3] = {21, 10, 0}, bits[3] = {11, 11, 10};
+#pragma unroll
   for (int pass = 0; pass < 3; ++pass) {
     const int sh = shift[pass], nb = 1 << bits[pass];
     for (int i = tid; i < nb; i += EV_NT) s_hist[i] = 0;
     __syncthreads();
-    for (int i = lo + tid; i < hi; i += EV_NT) {
-      const uint32_t key = evict_key(w[i]);
-      if ((key & mask) == prefix) atomicAdd(&s_hist[(key >> sh) & (nb - 1)], 1u);
-    }
+    sweep([&](int i, float x) {
+      const uint32_t key = evict_key(x);
+      if (i >= lo && i < hi && i < w1 && (key & mask) == prefix)
+        atomicAdd(&s_hist[(key >> sh) & (nb - 1)], 1u);
+    });
     __syncthreads();
     // The bin, from the top, in which the running count reaches `left`: thread t holds two
     // bins (the second histogram half is empty for 10 bits).
@@ -127,28 +153,23 @@ __global__ void __launch_bounds__(EV_NT) evict_select_kernel(EvictParams p) {
   // Keys above `prefix` are kept, of those equal to it the first `left`.  With nothing to
   // take, prefix is 0xffffffff: no key is above it, and left is 0.
 
-  // Each wave counts, then writes, its own run of [0, n), a multiple of 64 long.
-  const int run = ((n + EV_WAVES - 1) / EV_WAVES + 63) / 64 * 64;
-  const int w0 = wave * run, w1 = w0 + run < n ? w0 + run : n;
+  // Each wave counts, then writes, its own run.
   uint32_t above = 0, equal = 0;  // this lane's
-  for (int i = w0 + lane; i < w1; i += 64) {
-    const bool held = i < lo || i >= hi;
-    const uint32_t key = held ? 0 : evict_key(w[i]);
-    above += held || key > prefix;
-    equal += !held && key == prefix;
-  }
+  sweep([&](int i, float x) {
+    const bool live = i < w1, held = i < lo || i >= hi;
+    const uint32_t key = evict_key(x);
+    above += live && (held || key > prefix);
+    equal += live && !held && key == prefix;
+  });
   for (int o = 32; o; o >>= 1) above += __shfl_xor(above, o), equal += __shfl_xor(equal, o);
   if (lane == 0) s_wave[wave] = above, s_wave2[wave] = equal;
   __syncthreads();
   uint32_t at = 0, ties = 0;  // kept, and ties met, before this wave's run
   for (int k = 0; k < wave; ++k) at += s_wave[k], ties += s_wave2[k];
   at += ties < left ? ties : left;
-  for (int i0 = w0; i0 < w1; i0 += 64) {
-    const int i = i0 + lane;
-    const bool live = i < w1;
-    const bool held = live && (i < lo || i >= hi);
-    const float f = live ? w[i] : 0.0f;
-    const uint32_t key = evict_key(f);
+  sweep([&](int i, float x) {
+    const bool live = i < w1, held = live && (i < lo || i >= hi);
+    const uint32_t key = evict_key(x);
     const bool tie = live && !held && key == prefix;
     const uint64_t tb = __ballot(tie), below = ((uint64_t)1 << lane) - 1;
     const bool take = held || (live && !held && key > prefix) ||
@@ -157,37 +178,54 @@ __global__ void __launch_bounds__(EV_NT) evict_select_kernel(EvictParams p) {
     if (take) {
       const uint32_t o = at + (uint32_t)__popcll(kb & below);
       idx[o] = i;
-      wo[o] = f;
+      wo[o] = x;
     }
     at += (uint32_t)__popcll(kb);
     ties += (uint32_t)__popcll(tb);
-  }
+  });
 }
 
-// One thread per 16 bytes (VEC) or 2 bytes of a row: rows of the output in order, so a wave
-// writes neighbouring addresses.
+// One thread per 16 bytes (or 2 bytes, where rows are not aligned) of a row of the output in
+// order, so a wave writes neighbouring addresses; a workgroup takes EV_MOVE_STEPS turns.
+constexpr int EV_MOVE_STEPS = 4;
+
 template <class T>
-__global__ void __launch_bounds__(EV_MOVE_NT) evict_move_kernel(EvictParams p, int64_t items,
-                                                                int rows) {
-  const int per_row = p.row_bytes / (int)sizeof(T);
-  for (int64_t it = (int64_t)blockIdx.x * EV_MOVE_NT + threadIdx.x; it < items;
-       it += (int64_t)gridDim.x * EV_MOVE_NT) {
-    const int c = (int)(it % per_row);
-    const int64_t r = it / per_row;
-    const int h = (int)(r % p.H);
-    const int64_t r2 = r / p.H;
-    const int o = (int)(r2 % rows), b = (int)(r2 / rows);
-    const int64_t at = c * (int64_t)sizeof(T);
-    const int src = o < p.m ? p.index[((int64_t)b * p.H + h) * p.m + o] : -1;
-    T kv{}, vv{};
-    if (src >= 0) {
-      kv = *(const T*)(p.k + b * p.ksb + src * p.kst + h * p.ksh + at);
-      vv = *(const T*)(p.v + b * p.vsb + src * p.vst + h * p.vsh + at);
-    } else if (!p.zero_tail) {
-      continue;
+__global__ void __launch_bounds__(EV_MOVE_NT) evict_move_kernel(EvictParams p, LaunchDiv by_row,
+                                                                LaunchDiv by_heads, int rows) {
+  const int b = blockIdx.y;
+  const uint32_t items = (uint32_t)rows * by_heads.d * by_row.d;
+  const char *k = p.k + b * p.ksb, *v = p.v + b * p.vsb;
+  char *ko = p.k_out + b * p.kob, *vo = p.v_out + b * p.vob;
+  const uint32_t it0 = blockIdx.x * (EV_MOVE_NT * EV_MOVE_STEPS) + threadIdx.x;
+  int src[EV_MOVE_STEPS];
+  uint32_t r[EV_MOVE_STEPS], c[EV_MOVE_STEPS];
+#pragma unroll
+  for (int u = 0; u < EV_MOVE_STEPS; ++u) {
+    const uint32_t it = it0 + u * EV_MOVE_NT;
+    r[u] = by_row.div(it);
+    c[u] = it - r[u] * by_row.d;
+    const uint32_t o = by_heads.div(r[u]), h = r[u] - o * by_heads.d;
+    src[u] = -1;
+    if (it < items && o < (uint32_t)p.m) src[u] = p.index[((int64_t)b * p.H + h) * p.m + o];
+  }
+  T kv[EV_MOVE_STEPS], vv[EV_MOVE_STEPS];
+#pragma unroll
+  for (int u = 0; u < EV_MOVE_STEPS; ++u) {
+    const uint32_t o = by_heads.div(r[u]), h = r[u] - o * by_heads.d;
+    const int64_t at = c[u] * (int64_t)sizeof(T);
+    kv[u] = vv[u] = T{};
+    if (src[u] >= 0) {
+      kv[u] = *(const T*)(k + src[u] * p.kst + h * p.ksh + at);
+      vv[u] = *(const T*)(v + src[u] * p.vst + h * p.vsh + at);
     }
-    *(T*)(p.k_out + b * p.kob + o * p.kot + h * p.koh + at) = kv;
-    *(T*)(p.v_out + b * p.vob + o * p.vot + h * p.voh + at) = vv;
+  }
+#pragma unroll
+  for (int u = 0; u < EV_MOVE_STEPS; ++u) {
+    const uint32_t o = by_heads.div(r[u]), h = r[u] - o * by_heads.d;
+    if (it0 + u * EV_MOVE_NT >= items || (src[u] < 0 && !p.zero_tail)) continue;
+    const int64_t at = c[u] * (int64_t)sizeof(T);
+    *(T*)(ko + o * p.kot + h * p.koh + at) = kv[u];
+    *(T*)(vo + o * p.vot + h * p.voh + at) = vv[u];
   }
 }
 
@@ -204,6 +242,9 @@ extern "C" int nsmoe_cache_evict(const nsmoe_evict_args* a, void* stream) {
                 "cache_evict: bad batch, heads or head_dim");
   NSMOE_REQUIRE(a->cap >= 0 && a->cap < (1 << 30) && a->out_cap >= 0 && a->out_cap < (1 << 30),
                 "cache_evict: bad capacity");
+  NSMOE_REQUIRE(a->batch <= 65535 && a->out_cap * a->n_kv_heads * a->head_dim < (1ll << 31) - 4096,
+                "cache_evict: batch %lld (at most 65535) or a sequence's output (2^31 elements) "
+                "too large", (long long)a->batch);
   NSMOE_REQUIRE(a->budget >= 1 && a->budget <= a->out_cap,
                 "cache_evict: budget %lld outside 1 .. the output's %lld rows",
                 (long long)a->budget, (long long)a->out_cap);
@@ -260,13 +301,12 @@ extern "C" int nsmoe_cache_evict(const nsmoe_evict_args* a, void* stream) {
   NSMOE_TRY(check_launch("evict_select_kernel"));
   const int rows = P.zero_tail ? (int)P.So : P.m;
   const bool vec = (bits & 15) == 0;
-  const int64_t items = (int64_t)P.B * rows * P.H * (P.row_bytes / (vec ? 16 : 2));
-  int64_t grid = cdiv(items, EV_MOVE_NT);
-  const int64_t most = 16 * (int64_t)device_cus();
-  if (grid > most) grid = most;
+  const LaunchDiv by_row = launch_div(P.row_bytes / (vec ? 16 : 2)), by_heads = launch_div(P.H);
+  const dim3 grid((unsigned)cdiv((int64_t)rows * P.H * by_row.d, EV_MOVE_NT * EV_MOVE_STEPS),
+                  (unsigned)P.B);
   KernelTimer timer("evict_move", s);
-  if (vec) evict_move_kernel<u32x4><<<(unsigned)grid, EV_MOVE_NT, 0, s>>>(P, items, rows);
-  else evict_move_kernel<uint16_t><<<(unsigned)grid, EV_MOVE_NT, 0, s>>>(P, items, rows);
+  if (vec) evict_move_kernel<u32x4><<<grid, EV_MOVE_NT, 0, s>>>(P, by_row, by_heads, rows);
+  else evict_move_kernel<uint16_t><<<grid, EV_MOVE_NT, 0, s>>>(P, by_row, by_heads, rows);
   timer.stop();
   return check_launch("evict_move_kernel");
 }

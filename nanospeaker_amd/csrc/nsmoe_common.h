@@ -215,6 +215,20 @@ __device__ __forceinline__ float unpack2(uint32_t u, int e) {
   else return f16_to_f(v);
 }
 
+// ---- division by a divisor that a whole launch shares --------------------------------------
+//
+// The high half of a product with floor(2^32 / d) is the quotient or one less; one correction.
+struct LaunchDiv {
+  uint32_t d, mul;
+  __device__ __forceinline__ uint32_t div(uint32_t n) const {
+    const uint32_t q = __umulhi(n, mul);
+    return n - q * d >= d ? q + 1 : q;
+  }
+};
+inline LaunchDiv launch_div(int64_t d) {  // 1 <= d < 2^32
+  return LaunchDiv{(uint32_t)d, d == 1 ? 0xffffffffu : (uint32_t)((1ull << 32) / (uint64_t)d)};
+}
+
 // ---- wave helpers ---------------------------------------------------------------------
 
 __device__ __forceinline__ int lane_id() { return __lane_id(); }
