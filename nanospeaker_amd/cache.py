@@ -202,7 +202,7 @@ def cache_evict(k: Tensor, v: Tensor, weights: Tensor, lens: Tensor, budget: int
                 _fail(op, "out shares memory with the inputs or with itself")
             if not _writable(t):
                 _fail(op, "out has elements that share memory")
-    for t in (k, v, k_out, v_out, weights, w_out):
+    for t in (k, v, weights) if out is None else (k, v, weights, *out):
         if t.stride(-1) != 1 and t.shape[-1] > 1 and t.numel():
             _fail(op, "the last dim must be contiguous")
     index = torch.empty((b, hk, budget), dtype=torch.int32, device=dev)
@@ -210,9 +210,9 @@ def cache_evict(k: Tensor, v: Tensor, weights: Tensor, lens: Tensor, budget: int
     if b and hk and d:
         a = nat.evict_args(
             k.element_size(), hk, d, out is None, b, s, rows, budget, recent, sinks,
-            k.data_ptr(), v.data_ptr(), k_out.data_ptr(), v_out.data_ptr(), *_strides(k),
-            *_strides(v), *_strides(k_out), *_strides(v_out), weights.data_ptr(),
-            w_out.data_ptr(), *_strides(weights), *_strides(w_out), lens.data_ptr(),
+            k.data_ptr(), v.data_ptr(), k_out.data_ptr(), v_out.data_ptr(), *k.stride()[:3],
+            *v.stride()[:3], *k_out.stride()[:3], *v_out.stride()[:3], weights.data_ptr(),
+            w_out.data_ptr(), *weights.stride()[:2], *w_out.stride()[:2], lens.data_ptr(),
             lens_out.data_ptr(), index.data_ptr())
         with on_device(dev):
             nat.check(nat.lib().nsmoe_cache_evict(a, _stream(dev.index)), "nsmoe_cache_evict")
