@@ -49,7 +49,7 @@ int32_t nsmoe_abi_version(void);
  * "expert_bwd", "expert_dx", "dw" (or "dw_in" and "dw_out" where they run apart),
  * "combine_dx", "router_dw", "route_bwd", "norm_bwd", "attn_k_prep", "attn_fwd", "ce_rows", "norm_fwd", "rope",
  * "logits", "evict_select", "evict_move",
- * "prefix_part", "own_part", "prefix_join") until
+ * "prefix_part", "prefix_join") until
  * `capacity` pairs are used.
  * nsmoe_timing_read waits for the recorded events of one kernel and returns their
  * summed duration.  capacity 0 disables timing and frees the events. */

@@ -28,6 +28,8 @@
 // tiles that LDS-DMA copied with a chunk swizzle.  Scores, maxima, sums and outputs are fp32;
 // the probabilities enter the P V product rounded to the type (relative error up to half a
 // step each, of the size of the output's own rounding), their sum is of the unrounded ones.
+#include <algorithm>
+
 #include "../../include/nsmoe.h"
 #include "gemm_core.h"
 #include "nsmoe_capi_internal.h"
@@ -56,6 +58,7 @@ struct PrefixAttnParams {
   int chunk_p, chunk_s;  // keys per part
   int rbp, rbs;          // column blocks of a prefix part and of an own part
   int items_p;           // workgroups of the prefix (before the own ones)
+  LaunchDiv by_G, by_n;
   float scale_log2;
 };
 
@@ -119,34 +122,66 @@ __device__ __forceinline__ PartJob pa_job(const PrefixAttnParams& p, int item, b
 // A column of a part: which row of q / out it is, and the keys [first, last] it sees, in the
 // part's own numbering (none: last < first).
 struct Column {
-  int64_t row;  // (b n + i) Hq + head, or -1 past the last column
-  int64_t q;    // element offset into q
+  int row;    // (b n + i) Hq + head, or -1 past the last column
+  int64_t q;  // element offset into q
   int first, last;
 };
+
+// The keys that the query standing at row `at` of its cache sees, of the prefix or its own.
+__device__ __forceinline__ void pa_sight(const PrefixAttnParams& p, bool own, int at, int& first,
+                                         int& last) {
+  const int me = own ? at : p.P + at;
+  first = p.window ? max(0, me - p.window + 1) : 0;
+  last = own ? at : p.P - 1;
+  if (at < 0 || first > last) first = 0, last = -1;  // a query that has no row sees nothing
+}
 
 __device__ __forceinline__ Column pa_column(const PrefixAttnParams& p, const PartJob& j, int c) {
   Column r{-1, 0, 0, -1};
   if (c >= j.cols) return r;
-  const int g = c % p.G;
-  int i = c / p.G, b = j.b;
+  int i = (int)p.by_G.div(c), b = j.b;
+  const int head = j.hk * p.G + c - i * p.G;
   if (b < 0) {
-    b = i / p.n;
+    b = (int)p.by_n.div(i);
     i -= b * p.n;
   }
-  const int head = j.hk * p.G + g;
-  r.row = ((int64_t)b * p.n + i) * p.Hq + head;
+  r.row = (b * p.n + i) * p.Hq + head;
   r.q = b * p.qb + i * p.qn + head * p.qh;
-  const int at = pa_len(p, b) - p.n + i;  // the query's own row
-  if (at < 0) return r;                   // a query that has no row sees nothing
-  if (j.b < 0) {
-    r.last = p.P - 1;
-    r.first = p.window ? max(0, p.P + at - p.window + 1) : 0;
-  } else {
-    r.last = at;
-    r.first = p.window ? max(0, at - p.window + 1) : 0;
-  }
-  if (r.first > r.last) r.first = 0, r.last = -1;
+  pa_sight(p, j.b >= 0, pa_len(p, b) - p.n + i, r.first, r.last);
   return r;
+}
+
+// The keys [lo, hi) that some column of [col0, col0 + width) sees, within the part's.  Known
+// without the columns where nothing but the part decides it, so that the first tiles can be on
+// their way before the columns are looked at.
+__device__ __forceinline__ void pa_range(const PrefixAttnParams& p, const PartJob& j, int width,
+                                         int lane, int& lo, int& hi) {
+  if (j.b >= 0) {  // one sequence: its columns are in the order of their queries
+    const int at0 = pa_len(p, j.b) - p.n;
+    int first, last;
+    pa_sight(p, true, at0 + (int)p.by_G.div(min(j.col0 + width, j.cols) - 1), first, last);
+    hi = last + 1;
+    pa_sight(p, true, max(0, at0 + (int)p.by_G.div(j.col0)), lo, last);
+  } else if (!p.window) {
+    lo = 0;
+    hi = p.P;
+  } else {
+    lo = INT32_MAX;
+    hi = 0;
+    for (int c = j.col0 + lane; c < min(j.col0 + width, j.cols); c += 64) {
+      const Column k = pa_column(p, j, c);
+      if (k.last < k.first) continue;
+      lo = min(lo, k.first);
+      hi = max(hi, k.last + 1);
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      lo = min(lo, __shfl_xor(lo, o));
+      hi = max(hi, __shfl_xor(hi, o));
+    }
+  }
+  lo = __builtin_amdgcn_readfirstlane(max(lo, j.key0));
+  hi = __builtin_amdgcn_readfirstlane(min(hi, j.key1));
 }
 
 // Chunk swizzle of a row of 2 D bytes (D / 8 chunks of 16): chunk c of row r sits at slot
@@ -175,48 +210,45 @@ struct PaState {
   float m[NB], l[NB];
 };
 
-// The columns of a wave: query fragments and key ranges.
-template <int DT, int D, int NB>
+// The columns of a wave: query fragments, rows and key ranges.  SCORES: a form that calls with
+// accumulated weights use (up to 64 columns), which leaves the scores of own rows behind.
+template <int DT, int D, int NB, bool SCORES>
 struct PaCols {
   typename Mma<DT>::Frag q[NB][D / 32];
-  int first[NB], last[NB];
+  int row[NB], first[NB], last[NB];
+  float* score[SCORES ? NB : 1];  // this lane's column's scores (from key 0 on), or NULL
 };
 
-template <int DT, int D, int NB>
+template <int DT, int D, int NB, bool SC>
 __device__ __forceinline__ void pa_load_cols(const PrefixAttnParams& p, const PartJob& j, int c0,
-                                             int lane, PaCols<DT, D, NB>& w, int& lo, int& hi) {
+                                             int lane, PaCols<DT, D, NB, SC>& w) {
   const int l16 = lane & 15, g = lane >> 4;
-  lo = INT32_MAX;
-  hi = 0;
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
-    const Column c = pa_column(p, j, c0 + 16 * nb + l16);
+    const int col = c0 + 16 * nb + l16;
+    const Column c = pa_column(p, j, col);
+    const bool live = c.last >= c.first;
+    w.row[nb] = c.row;
     w.first[nb] = c.first;
     w.last[nb] = c.last;
-    const bool live = c.last >= c.first;
-    if (live) {
-      lo = min(lo, c.first);
-      hi = max(hi, c.last + 1);
-    }
+    if (c.row < 0) w.last[nb] = INT32_MAX;  // a padding column asks for no mask
 #pragma unroll
     for (int ks = 0; ks < D / 32; ++ks) {
       u32x4 v = {0u, 0u, 0u, 0u};
       if (live) v = *(const u32x4*)(p.q + c.q + 32 * ks + 8 * g);
       w.q[nb][ks].v = v;
     }
+    if constexpr (SC)
+      w.score[nb] = p.score && j.b >= 0 && c.row >= 0
+                        ? p.score + (((int64_t)j.b * p.Hkv + j.hk) * j.cols + col) * p.spad
+                        : nullptr;
   }
-#pragma unroll
-  for (int o = 1; o < 16; o <<= 1) {
-    lo = min(lo, __shfl_xor(lo, o));
-    hi = max(hi, __shfl_xor(hi, o));
-  }
-  lo = min(lo, hi);  // nothing seen: an empty range
 }
 
 // A tile of KB * 16 keys from key0 on, in three steps.  Scores: S^T = K Q^T from the K rows in
 // LDS; lane (g, l16) gets keys 16 kb + 4 g + e of column l16.
-template <int DT, int D, int NB, int KB>
-__device__ __forceinline__ void pa_scores(const PaCols<DT, D, NB>& w, const char* Kt, int lane,
+template <int DT, int D, int NB, int KB, bool SC>
+__device__ __forceinline__ void pa_scores(const PaCols<DT, D, NB, SC>& w, const char* Kt, int lane,
                                           f32x4 (&s)[KB][NB]) {
   using M = Mma<DT>;
   constexpr int RB = 2 * D;  // bytes per row
@@ -236,12 +268,11 @@ __device__ __forceinline__ void pa_scores(const PaCols<DT, D, NB>& w, const char
     }
 }
 
-// Masks, then turns the scores into probabilities against the running maximum.  `score`: where
-// to leave this lane's column's scaled scores (the tile's key 0), or NULL per block.
-template <int DT, int D, int NB, int KB>
-__device__ __forceinline__ void pa_softmax(const PaCols<DT, D, NB>& w, PaState<D, NB>& st,
-                                           f32x4 (&s)[KB][NB], int key0, float c, int lane,
-                                           float* const (&score)[NB]) {
+// Masks, leaves the scaled scores where they are asked for, then turns them into
+// probabilities against the running maximum.
+template <int DT, int D, int NB, int KB, bool SC>
+__device__ __forceinline__ void pa_softmax(const PaCols<DT, D, NB, SC>& w, PaState<D, NB>& st,
+                                           f32x4 (&s)[KB][NB], int key0, float c, int lane) {
   const int g = lane >> 4;
   // Keys outside a column's range: one select per score, on tiles that cross some edge only.
   bool edge = false;
@@ -261,9 +292,12 @@ __device__ __forceinline__ void pa_softmax(const PaCols<DT, D, NB>& w, PaState<D
   }
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
-    if (score[nb]) {
+    if constexpr (SC) {
+      if (w.score[nb]) {
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb) *(f32x4*)(score[nb] + 16 * kb + 4 * g) = s[kb][nb] * c;
+        for (int kb = 0; kb < KB; ++kb)
+          *(f32x4*)(w.score[nb] + key0 + 16 * kb + 4 * g) = s[kb][nb] * c;
+      }
     }
     float mx = st.m[nb];
 #pragma unroll
@@ -406,26 +440,11 @@ __device__ void pa_few(const PrefixAttnParams& p, const PartJob& j, char* lds) {
   constexpr int NC = TILE / 1024;  // copies of one of K / V per tile
   const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  PaCols<DT, D, NB> w;
   int lo, hi;
-  pa_load_cols<DT, D, NB>(p, j, j.col0, lane, w, lo, hi);
-  lo = __builtin_amdgcn_readfirstlane(max(lo, j.key0));
-  hi = __builtin_amdgcn_readfirstlane(min(hi, j.key1));
-  float* score[NB];
-#pragma unroll
-  for (int nb = 0; nb < NB; ++nb) {
-    const int col = j.col0 + 16 * nb + l16;
-    score[nb] = p.score && j.b >= 0 && col < j.cols
-                    ? p.score + (((int64_t)j.b * p.Hkv + j.hk) * j.cols + col) * p.spad
-                    : nullptr;
-    // Padding columns see nothing and ask for no mask.
-    if (col >= j.cols) w.first[nb] = 0, w.last[nb] = INT32_MAX;
-  }
+  pa_range(p, j, 16 * NB, lane, lo, hi);
   // One buffer each for K and V, a wave's own: the next tile's K is copied from when this
   // one's scores are done, its V from when this one's product is.  What hides the copies'
   // latency is the other waves of the CU (8 to 16, each with 8 or 16 KiB of tile).
-  PaState<D, NB> st;
-  pa_clear(st);
   char* Kt = lds + wave * 2 * TILE;
   char* Vt = Kt + TILE;
   const uint32_t kd = pa_lds(Kt), vd = kd + TILE;
@@ -438,19 +457,20 @@ __device__ void pa_few(const PrefixAttnParams& p, const PartJob& j, char* lds) {
     ck.issue(t * KEYS, KEYS, lo, hi, kd, lane);
     cv.issue(t * KEYS, KEYS, lo, hi, vd, lane);
   }
+  PaCols<DT, D, NB, true> w;
+  pa_load_cols(p, j, j.col0, lane, w);
+  PaState<D, NB> st;
+  pa_clear(st);
   for (; t < t1; t += 4) {
     f32x4 s[KB][NB];
     wait_vmcnt<NC>();  // this tile's K; its V stays in flight
     asm volatile("" ::: "memory");
-    pa_scores<DT, D, NB, KB>(w, Kt, lane, s);
+    pa_scores(w, Kt, lane, s);
     asm volatile("" ::: "memory");
     wait_lgkm0();      // K has been read
     const bool more = t + 4 < t1;
     if (more) ck.issue((t + 4) * KEYS, KEYS, lo, hi, kd, lane);
-    float* sc[NB];
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb) sc[nb] = score[nb] ? score[nb] + t * KEYS : nullptr;
-    pa_softmax<DT, D, NB, KB>(w, st, s, t * KEYS, p.scale_log2, lane, sc);
+    pa_softmax(w, st, s, t * KEYS, p.scale_log2, lane);
     if (more) wait_vmcnt<NC>();  // this tile's V; the next K stays in flight
     else wait_vmcnt<0>();
     asm volatile("" ::: "memory");
@@ -464,6 +484,7 @@ __device__ void pa_few(const PrefixAttnParams& p, const PartJob& j, char* lds) {
   float* s_o = (float*)lds;                     // [4][16][D]
   float* s_m = (float*)(lds + 4 * 16 * D * 4);  // [4][16]
   float* s_l = s_m + 4 * 16;                    // [4][16]
+  int* s_row = (int*)(s_l + 4 * 16);            // [16]
   const int slots = p.np + p.ns;
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
@@ -474,6 +495,7 @@ __device__ void pa_few(const PrefixAttnParams& p, const PartJob& j, char* lds) {
     if (g == 0) {
       s_m[wave * 16 + l16] = st.m[nb];
       s_l[wave * 16 + l16] = l;
+      s_row[l16] = w.row[nb];
     }
 #pragma unroll
     for (int db = 0; db < D / 16; ++db)
@@ -481,12 +503,12 @@ __device__ void pa_few(const PrefixAttnParams& p, const PartJob& j, char* lds) {
     __syncthreads();
     for (int i = threadIdx.x; i < 16 * (D / 4); i += PA_NT) {
       const int col = i / (D / 4), d = (i % (D / 4)) * 4;
-      const Column c = pa_column(p, j, j.col0 + 16 * nb + col);
-      if (c.row < 0) continue;
+      const int row = s_row[col];
+      if (row < 0) continue;
       float m = PA_NONE;
 #pragma unroll
       for (int k = 0; k < 4; ++k) m = fmaxf(m, s_m[k * 16 + col]);
-      const int64_t at = c.row * slots + j.slot;
+      const int64_t at = (int64_t)row * slots + j.slot;
       f32x4 o = {0.f, 0.f, 0.f, 0.f};
       float sum = 0.0f;
       if (m != PA_NONE) {
@@ -513,27 +535,8 @@ __device__ void pa_many(const PrefixAttnParams& p, const PartJob& j, char* lds) 
   constexpr int NC = TILE / 1024 / 4;  // copies of one of K / V per tile and wave
   const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  PaCols<DT, D, NB> w;
   int lo, hi;
-  const int c0 = j.col0 + wave * 16 * NB;
-  pa_load_cols<DT, D, NB>(p, j, c0, lane, w, lo, hi);
-  int* s_lo = (int*)lds;  // [4], then s_hi[4]
-  if (lane == 0) s_lo[wave] = hi > lo ? lo : INT32_MAX, s_lo[4 + wave] = hi;
-  __syncthreads();
-  lo = min(min(s_lo[0], s_lo[1]), min(s_lo[2], s_lo[3]));
-  hi = max(max(s_lo[4], s_lo[5]), max(s_lo[6], s_lo[7]));
-  lo = __builtin_amdgcn_readfirstlane(max(lo, j.key0));
-  hi = __builtin_amdgcn_readfirstlane(min(hi, j.key1));
-  __syncthreads();  // before the first copies land there
-  float* score[NB];
-#pragma unroll
-  for (int nb = 0; nb < NB; ++nb) {
-    const int col = c0 + 16 * nb + l16;
-    score[nb] = p.score && j.b >= 0 && col < j.cols
-                    ? p.score + (((int64_t)j.b * p.Hkv + j.hk) * j.cols + col) * p.spad
-                    : nullptr;
-    if (col >= j.cols) w.first[nb] = 0, w.last[nb] = INT32_MAX;
-  }
+  pa_range(p, j, 64 * NB, lane, lo, hi);
   const uint32_t lds0 = pa_lds(lds) + (uint32_t)(wave * NC * 1024);
   PaCopy<D, NC> ck, cv;
   constexpr int ROWS = KEYS / 4;  // rows that a wave copies
@@ -544,12 +547,14 @@ __device__ void pa_many(const PrefixAttnParams& p, const PartJob& j, char* lds) 
     ck.issue(t * KEYS, KEYS, lo, hi, dst, lane);
     cv.issue(t * KEYS, KEYS, lo, hi, dst + TILE, lane);
   };
-  PaState<D, NB> st;
-  pa_clear(st);
   const int t0 = hi > lo ? lo / KEYS : 0, t1 = hi > lo ? (hi + KEYS - 1) / KEYS : 0;
 #pragma unroll
   for (int u = 0; u < ST - 1; ++u)
     if (t0 + u < t1) issue(t0 + u, u);
+  PaCols<DT, D, NB, NB == 1> w;
+  pa_load_cols(p, j, j.col0 + wave * 16 * NB, lane, w);
+  PaState<D, NB> st;
+  pa_clear(st);
   int stage = 0;
   for (int t = t0; t < t1; ++t) {
     // this wave's copies of tile t; with three stages tile t + 1's stay in flight
@@ -560,12 +565,9 @@ __device__ void pa_many(const PrefixAttnParams& p, const PartJob& j, char* lds) 
     barrier_dma();  // every wave's copies of tile t; every wave done with tile t - 1
     if (t + ST - 1 < t1) issue(t + ST - 1, (stage + ST - 1) % ST);
     const char* tile = lds + stage * 2 * TILE;
-    float* sc[NB];
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb) sc[nb] = score[nb] ? score[nb] + t * KEYS : nullptr;
     f32x4 s[KB][NB];
-    pa_scores<DT, D, NB, KB>(w, tile, lane, s);
-    pa_softmax<DT, D, NB, KB>(w, st, s, t * KEYS, p.scale_log2, lane, sc);
+    pa_scores(w, tile, lane, s);
+    pa_softmax(w, st, s, t * KEYS, p.scale_log2, lane);
     pa_values<DT, D, NB, KB, PA_SPLIT_MANY && DT == DT_BF16>(st, s, tile + TILE, lane);
     stage = stage + 1 == ST ? 0 : stage + 1;
   }
@@ -576,9 +578,8 @@ __device__ void pa_many(const PrefixAttnParams& p, const PartJob& j, char* lds) 
     float l = st.l[nb];
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
-    const Column c = pa_column(p, j, c0 + 16 * nb + l16);
-    if (c.row < 0) continue;
-    const int64_t at = c.row * slots + j.slot;
+    if (w.row[nb] < 0) continue;
+    const int64_t at = (int64_t)w.row[nb] * slots + j.slot;
     if (g == 0) p.part_ml[at] = make_float2(st.m[nb] * p.scale_log2, l);
     if (st.m[nb] == PA_NONE) continue;
     float* dst = p.part_o + at * D + 4 * g;
@@ -730,30 +731,44 @@ static int pa_form(int64_t cols, int D) {
 
 static PrefixPlan pa_plan(const nsmoe_prefix_attn_args* a) {
   PrefixPlan pl{};
-  const int64_t G = a->n_heads / a->n_kv_heads, B = a->batch, n = a->n_new;
-  const int64_t slots = 2 * device_cus();  // workgroups that run at once
+  const int64_t G = a->n_heads / a->n_kv_heads, B = a->batch, n = a->n_new, D = a->head_dim;
+  const int64_t cus = device_cus(), slots = 2 * cus;  // workgroups that run at once
   pl.rows = B * n * a->n_heads;
   pl.form_p = a->prefix_len > 0 ? pa_form(B * n * G, a->head_dim) : -1;
   pl.form_s = a->cap > 0 ? pa_form(n * G, a->head_dim) : -1;
-  // Keys per part, whole tiles of all four waves: as few as give `per` parts for each slot,
-  // at least 128 (a tile a wave), and at most 64 parts.
-  auto chunk_of = [&](int64_t groups, int64_t keys, int64_t want) {
-    int64_t parts = want / groups;
+  // What the two kinds of parts take, roughly, in us on the whole chip: the bytes of their keys
+  // and values at 5 TB/s (the caches half full) or their products at 600 TFLOP/s.
+  auto cost = [&](double keys, double cols) {
+    return std::max(keys * a->n_kv_heads * D * 4 / 5e6, keys * cols * a->n_kv_heads * D * 4 / 6e8);
+  };
+  const double cost_p = cost((double)a->prefix_len, (double)(B * n * G));
+  const double cost_s = cost(0.5 * (double)(a->cap * B), (double)(n * G));
+  // Keys per part: whole turns of four 32-key tiles, at most 64 parts.
+  auto chunk_of = [&](int64_t keys, int64_t parts) {
     parts = parts < 1 ? 1 : parts > 64 ? 64 : parts;
-    int64_t c = cdiv(cdiv(keys, parts), 128) * 128;
-    return (int)c;
+    return (int)(cdiv(cdiv(keys, parts), 128) * 128);
   };
   if (pl.form_p >= 0) {
+    // The prefix's parts take their share of the chip beside the caches' (64 sequences behind
+    // 8192 rows, dim 128, 1024-row caches: 128 to 192 of 512 workgroups 53 us, 512 of them 70).
+    // Under many columns a part pays for its columns' loads and its output with 512 keys of
+    // work, or 256 while there are fewer parts than CUs (that prefix alone: 24 us at 512 keys
+    // a part, 33 at 1024, 27 at 256).
     pl.rbp = (int)cdiv(B * n * G, PA_WIDTH[pl.form_p]);
-    const int64_t groups = (int64_t)pl.rbp * a->n_kv_heads;
-    pl.chunk_p = chunk_of(groups, a->prefix_len, pl.form_p < 2 ? 4 * slots : slots);
-    pl.np = (int)cdiv(a->prefix_len, pl.chunk_p);
+    const int64_t groups = (int64_t)pl.rbp * a->n_kv_heads, keys = a->prefix_len;
+    int64_t parts = (int64_t)((double)slots * cost_p / (cost_p + cost_s) / groups + 0.5);
+    if (pl.form_p < 2) parts *= 2;
+    else parts = std::min(parts, std::max(keys / 512, std::min(keys / 256, cus / groups)));
+    pl.chunk_p = chunk_of(keys, parts);
+    pl.np = (int)cdiv(keys, pl.chunk_p);
     pl.items_p = pl.np * groups;
   }
   if (pl.form_s >= 0) {
+    // Two parts a slot even ragged lengths out; a part's start and end cost about 2 us, so
+    // more lose (64 x 640 rows, dim 128: 37 us, 35 with one part, 40 with four).
     pl.rbs = (int)cdiv(n * G, PA_WIDTH[pl.form_s]);
     const int64_t groups = B * pl.rbs * a->n_kv_heads;
-    pl.chunk_s = chunk_of(groups, a->cap, 4 * slots);
+    pl.chunk_s = chunk_of(a->cap, 2 * slots / groups);
     pl.ns = (int)cdiv(a->cap, pl.chunk_s);
     pl.items_s = pl.ns * groups;
   }
@@ -768,14 +783,15 @@ static PrefixPlan pa_plan(const nsmoe_prefix_attn_args* a) {
 }
 
 template <int DT, int D, int FP, int FS>
-static int pa_run(const PrefixAttnParams& P, int64_t items, const char* name, hipStream_t s) {
+static int pa_run(const PrefixAttnParams& P, int64_t items, hipStream_t s) {
   constexpr int few = PaGeo<D>::FEW_LDS, many = PaGeo<D>::MANY_LDS;
   constexpr int lds = (FP >= 2 || FS >= 2) && many > few ? many
                       : (FP >= 0 && FP < 2) || (FS >= 0 && FS < 2) ? few : many;
+  static_assert(PA_WIDTH[2] == 64, "weights stay within the forms that keep scores");
   static_assert(2 * 64 <= PA_MAX_SLOTS, "a lane holds two slots");
-  static_assert(4 * 16 * (D * 4 + 8) <= few, "the join of the waves fits their buffers");
+  static_assert(4 * 16 * (D * 4 + 8) + 64 <= few, "the join of the waves fits their buffers");
   NSMOE_REQUIRE(items < INT32_MAX, "prefix_attention: grid too large");
-  KernelTimer timer(name, s);
+  KernelTimer timer("prefix_part", s);
   prefix_part_kernel<DT, D, FP, FS><<<(unsigned)items, PA_NT, lds, s>>>(P);
   timer.stop();
   return check_launch("prefix_part_kernel");
@@ -797,24 +813,24 @@ static int pa_with_form(int form, F&& f) {
 
 template <int DT, int D>
 static int pa_launch(const PrefixAttnParams& P, const PrefixPlan& pl, hipStream_t s) {
-  // Own caches under few columns (a decode step) share the prefix's launch; under many they
-  // are a launch of their own.
-  if (pl.form_p >= 0 && pl.form_s >= 0 && pl.form_s < 2) {
-    const int64_t items = pl.items_p + pl.items_s;
+  // One launch for both kinds (a cache's columns are some of the prefix's: FS <= FP).
+  const int64_t items = pl.items_p + pl.items_s;
+  if (pl.form_p >= 0 && pl.form_s >= 0) {
     NSMOE_TRY(pa_with_form<D>(pl.form_p, [&](auto fp) {
-      constexpr int FP = decltype(fp)::value;
-      return pl.form_s == 0 ? pa_run<DT, D, FP, 0>(P, items, "prefix_part", s)
-                            : pa_run<DT, D, FP, 1>(P, items, "prefix_part", s);
+      return pa_with_form<D>(pl.form_s, [&](auto fs) {
+        constexpr int FP = decltype(fp)::value, FS = decltype(fs)::value;
+        if constexpr (FS <= FP) return pa_run<DT, D, FP, FS>(P, items, s);
+        else return (int)NSMOE_EINVAL;
+      });
     }));
-  } else {
-    if (pl.form_p >= 0)
-      NSMOE_TRY(pa_with_form<D>(pl.form_p, [&](auto fp) {
-        return pa_run<DT, D, decltype(fp)::value, -1>(P, pl.items_p, "prefix_part", s);
-      }));
-    if (pl.form_s >= 0)
-      NSMOE_TRY(pa_with_form<D>(pl.form_s, [&](auto fs) {
-        return pa_run<DT, D, -1, decltype(fs)::value>(P, pl.items_s, "own_part", s);
-      }));
+  } else if (pl.form_p >= 0) {
+    NSMOE_TRY(pa_with_form<D>(pl.form_p, [&](auto fp) {
+      return pa_run<DT, D, decltype(fp)::value, -1>(P, items, s);
+    }));
+  } else if (pl.form_s >= 0) {
+    NSMOE_TRY(pa_with_form<D>(pl.form_s, [&](auto fs) {
+      return pa_run<DT, D, -1, decltype(fs)::value>(P, items, s);
+    }));
   }
   const int64_t row_blocks = cdiv(pl.rows, 4);
   int64_t grid = row_blocks;
@@ -924,6 +940,8 @@ extern "C" int nsmoe_prefix_attention(const nsmoe_prefix_attn_args* a, void* wor
   P.rbp = pl.rbp;
   P.rbs = pl.rbs;
   P.items_p = (int)pl.items_p;
+  P.by_G = launch_div(P.G);
+  P.by_n = launch_div(P.n);
   P.scale_log2 = a->scale * 1.4426950408889634f;
   hipStream_t s = (hipStream_t)stream;
   if (a->head_dim == 64)
