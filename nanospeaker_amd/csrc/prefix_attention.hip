@@ -210,6 +210,9 @@ struct PaState {
   float m[NB], l[NB];
 };
 
+// A column's row, -1 for a padding column, PA_BLIND - row for one that sees nothing here.
+constexpr int PA_BLIND = -2;
+
 // The columns of a wave: query fragments, rows and key ranges.  SCORES: a form that calls with
 // accumulated weights use (up to 64 columns), which leaves the scores of own rows behind.
 template <int DT, int D, int NB, bool SCORES>
@@ -228,10 +231,11 @@ __device__ __forceinline__ void pa_load_cols(const PrefixAttnParams& p, const Pa
     const int col = c0 + 16 * nb + l16;
     const Column c = pa_column(p, j, col);
     const bool live = c.last >= c.first;
-    w.row[nb] = c.row;
+    // A column that sees nothing, and a padding one, asks for no mask: its zero queries are
+    // multiplied like any other's and what comes of it is dropped at the end.
+    w.row[nb] = live || c.row < 0 ? c.row : PA_BLIND - c.row;
     w.first[nb] = c.first;
-    w.last[nb] = c.last;
-    if (c.row < 0) w.last[nb] = INT32_MAX;  // a padding column asks for no mask
+    w.last[nb] = live ? c.last : INT32_MAX;
 #pragma unroll
     for (int ks = 0; ks < D / 32; ++ks) {
       u32x4 v = {0u, 0u, 0u, 0u};
@@ -503,11 +507,13 @@ __device__ void pa_few(const PrefixAttnParams& p, const PartJob& j, char* lds) {
     __syncthreads();
     for (int i = threadIdx.x; i < 16 * (D / 4); i += PA_NT) {
       const int col = i / (D / 4), d = (i % (D / 4)) * 4;
-      const int row = s_row[col];
+      const int r = s_row[col], row = r <= PA_BLIND ? PA_BLIND - r : r;
       if (row < 0) continue;
       float m = PA_NONE;
+      if (r >= 0) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) m = fmaxf(m, s_m[k * 16 + col]);
+        for (int k = 0; k < 4; ++k) m = fmaxf(m, s_m[k * 16 + col]);
+      }
       const int64_t at = (int64_t)row * slots + j.slot;
       f32x4 o = {0.f, 0.f, 0.f, 0.f};
       float sum = 0.0f;
@@ -578,10 +584,12 @@ __device__ void pa_many(const PrefixAttnParams& p, const PartJob& j, char* lds) 
     float l = st.l[nb];
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
-    if (w.row[nb] < 0) continue;
-    const int64_t at = (int64_t)w.row[nb] * slots + j.slot;
-    if (g == 0) p.part_ml[at] = make_float2(st.m[nb] * p.scale_log2, l);
-    if (st.m[nb] == PA_NONE) continue;
+    const int r = w.row[nb], row = r <= PA_BLIND ? PA_BLIND - r : r;
+    if (row < 0) continue;
+    const int64_t at = (int64_t)row * slots + j.slot;
+    const float m = r >= 0 ? st.m[nb] : PA_NONE;
+    if (g == 0) p.part_ml[at] = make_float2(m * p.scale_log2, l);
+    if (m == PA_NONE) continue;
     float* dst = p.part_o + at * D + 4 * g;
 #pragma unroll
     for (int db = 0; db < D / 16; ++db) *(f32x4*)(dst + 16 * db) = st.o[db][nb];
