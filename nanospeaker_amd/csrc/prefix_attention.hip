@@ -272,37 +272,44 @@ __device__ __forceinline__ void pa_scores(const PaCols<DT, D, NB, SC>& w, const 
     }
 }
 
-// Masks, leaves the scaled scores where they are asked for, then turns them into
-// probabilities against the running maximum.
+// Keys outside a column's range: one select per score, on tiles that cross some edge only.
 template <int DT, int D, int NB, int KB, bool SC>
-__device__ __forceinline__ void pa_softmax(const PaCols<DT, D, NB, SC>& w, PaState<D, NB>& st,
-                                           f32x4 (&s)[KB][NB], int key0, float c, int lane) {
+__device__ __forceinline__ void pa_mask(const PaCols<DT, D, NB, SC>& w, f32x4 (&s)[KB][NB], int key0,
+                                        int lane) {
   const int g = lane >> 4;
-  // Keys outside a column's range: one select per score, on tiles that cross some edge only.
   bool edge = false;
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) edge |= w.first[nb] > key0 || w.last[nb] < key0 + 16 * KB - 1;
-  if (__ballot(edge)) {
+  if (!__ballot(edge)) return;
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
+  for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int key = key0 + 16 * kb + 4 * g + e;
+        const bool dead = (key < w.first[nb]) | (key > w.last[nb]);
+        s[kb][nb][e] = dead ? PA_NONE : s[kb][nb][e];
+      }
+}
+
+// Leaves a tile's scores where they are asked for.
+template <int DT, int D, int NB, int KB, bool SC>
+__device__ __forceinline__ void pa_keep(const PaCols<DT, D, NB, SC>& w, const f32x4 (&s)[KB][NB],
+                                        int key0, float c, int lane) {
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb)
+    if (w.score[nb])
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int key = key0 + 16 * kb + 4 * g + e;
-          const bool dead = (key < w.first[nb]) | (key > w.last[nb]);
-          s[kb][nb][e] = dead ? PA_NONE : s[kb][nb][e];
-        }
-  }
+        *(f32x4*)(w.score[nb] + key0 + 16 * kb + 4 * (lane >> 4)) = s[kb][nb] * c;
+}
+
+// Turns masked scores into probabilities against the running maximum.
+template <int D, int NB, int KB>
+__device__ __forceinline__ void pa_softmax(PaState<D, NB>& st, f32x4 (&s)[KB][NB], float c) {
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
-    if constexpr (SC) {
-      if (w.score[nb]) {
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
-          *(f32x4*)(w.score[nb] + key0 + 16 * kb + 4 * g) = s[kb][nb] * c;
-      }
-    }
     float mx = st.m[nb];
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
@@ -427,8 +434,9 @@ __device__ __forceinline__ uint32_t pa_lds(const char* p) {
   return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)p;
 }
 
+constexpr int FEW_KEYS_OF(int D) { return 32; }
 template <int D> struct PaGeo {
-  static constexpr int FEW_KEYS = 32;
+  static constexpr int FEW_KEYS = FEW_KEYS_OF(D);
   static constexpr int FEW_TILE = FEW_KEYS * 2 * D;  // bytes of K or V
   static constexpr int FEW_LDS = 4 * 2 * FEW_TILE;   // 32 or 64 KiB
   static constexpr int MANY_KEYS = 64;
@@ -465,16 +473,30 @@ __device__ void pa_few(const PrefixAttnParams& p, const PartJob& j, char* lds) {
   pa_load_cols(p, j, j.col0, lane, w);
   PaState<D, NB> st;
   pa_clear(st);
+  // Scores that are asked for are stored a tile late, after a wait that has given the copies
+  // time: stores count with the copies, and the waits below would stand still for fresh ones.
+  const bool keep = p.score && j.b >= 0;
+  f32x4 raw[KB][NB];
+  int raw_at = -1;
   for (; t < t1; t += 4) {
     f32x4 s[KB][NB];
     wait_vmcnt<NC>();  // this tile's K; its V stays in flight
     asm volatile("" ::: "memory");
+    if (keep && raw_at >= 0) pa_keep(w, raw, raw_at, p.scale_log2, lane);
     pa_scores(w, Kt, lane, s);
     asm volatile("" ::: "memory");
     wait_lgkm0();      // K has been read
     const bool more = t + 4 < t1;
     if (more) ck.issue((t + 4) * KEYS, KEYS, lo, hi, kd, lane);
-    pa_softmax(w, st, s, t * KEYS, p.scale_log2, lane);
+    pa_mask(w, s, t * KEYS, lane);
+    if (keep) {
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) raw[kb][nb] = s[kb][nb];
+      raw_at = t * KEYS;
+    }
+    pa_softmax(st, s, p.scale_log2);
     if (more) wait_vmcnt<NC>();  // this tile's V; the next K stays in flight
     else wait_vmcnt<0>();
     asm volatile("" ::: "memory");
@@ -483,6 +505,8 @@ __device__ void pa_few(const PrefixAttnParams& p, const PartJob& j, char* lds) {
     wait_lgkm0();      // V has been read
     if (more) cv.issue((t + 4) * KEYS, KEYS, lo, hi, vd, lane);
   }
+
+  if (keep && raw_at >= 0) pa_keep(w, raw, raw_at, p.scale_log2, lane);
 
   // Join the four waves through LDS, 16 columns at a time.
   float* s_o = (float*)lds;                     // [4][16][D]
@@ -573,7 +597,9 @@ __device__ void pa_many(const PrefixAttnParams& p, const PartJob& j, char* lds) 
     const char* tile = lds + stage * 2 * TILE;
     f32x4 s[KB][NB];
     pa_scores(w, tile, lane, s);
-    pa_softmax(w, st, s, t * KEYS, p.scale_log2, lane);
+    pa_mask(w, s, t * KEYS, lane);
+    if constexpr (NB == 1) pa_keep(w, s, t * KEYS, p.scale_log2, lane);
+    pa_softmax(st, s, p.scale_log2);
     pa_values<DT, D, NB, KB, PA_SPLIT_MANY && DT == DT_BF16>(st, s, tile + TILE, lane);
     stage = stage + 1 == ST ? 0 : stage + 1;
   }
@@ -699,24 +725,37 @@ __global__ void __launch_bounds__(PA_NT) prefix_join_kernel(PrefixAttnParams p, 
   for (int c = wave; c < cols; c += 4) {
     const PaTotal t =
         pa_total(p, ((int64_t)b * p.n + c / p.G) * p.Hq + hk * p.G + c % p.G, lane);
-    if (lane == 0) s_total[c] = t.m == PA_NONE ? INFINITY : t.m + log2f(t.l);  // 2^-inf = 0
+    if (lane == 0) s_total[c] = t.m == PA_NONE ? INFINITY : t.m + log2f(t.l);  // 2^(x - inf) = 0
   }
   __syncthreads();
-  const int row0 = pa_len(p, b) - p.n;
+  const int row0 = pa_len(p, b) - p.n, key0 = chunk * PA_JOIN_KEYS + threadIdx.x;
   const int64_t head = (int64_t)b * p.Hkv + hk;
+  constexpr int KPT = PA_JOIN_KEYS / PA_NT;
+  float sum[KPT], before[KPT];  // the new weights are added up before they meet the old
 #pragma unroll
-  for (int u = 0; u < PA_JOIN_KEYS / PA_NT; ++u) {
-    const int key = chunk * PA_JOIN_KEYS + u * PA_NT + threadIdx.x;
-    if (key >= p.S) return;
-    // Only the columns that see the key: their scores alone were written.
-    const float* sc = p.score + head * cols * p.spad + key;
-    float sum = 0.0f;
-    for (int c = 0; c < cols; ++c) {
-      const int at = row0 + c / p.G;
-      if (at >= key && (!p.window || at - key < p.window))
-        sum += __builtin_amdgcn_exp2f(sc[(int64_t)c * p.spad] - s_total[c]);
+  for (int u = 0; u < KPT; ++u) {
+    const int key = key0 + u * PA_NT;
+    before[u] = p.w_in && key < p.S ? p.w_in[head * p.S + key] : 0.0f;
+    sum[u] = 0.0f;
+  }
+  // Only the columns that see a key: their scores alone were written.
+  for (int c = 0; c < cols; ++c) {
+    const int at = row0 + (int)p.by_G.div(c);
+    const float* sc = p.score + (head * cols + c) * p.spad;
+    const float total = s_total[c];
+    float x[KPT];
+#pragma unroll
+    for (int u = 0; u < KPT; ++u) {
+      const int key = key0 + u * PA_NT;
+      x[u] = key <= at && (!p.window || at - key < p.window) ? sc[key] : PA_NONE;
     }
-    p.w_out[head * p.S + key] = (p.w_in ? p.w_in[head * p.S + key] : 0.0f) + sum;
+#pragma unroll
+    for (int u = 0; u < KPT; ++u) sum[u] += __builtin_amdgcn_exp2f(x[u] - total);
+  }
+#pragma unroll
+  for (int u = 0; u < KPT; ++u) {
+    const int key = key0 + u * PA_NT;
+    if (key < p.S) p.w_out[head * p.S + key] = before[u] + sum[u];
   }
 }
 
