@@ -471,6 +471,7 @@ __device__ void pa_few(const PrefixAttnParams& p, const PartJob& j, char* lds) {
   }
   PaCols<DT, D, NB, true> w;
   pa_load_cols(p, j, j.col0, lane, w);
+  wait_vmcnt<0>();  // see pa_many
   PaState<D, NB> st;
   pa_clear(st);
   // Scores that are asked for are stored a tile late, after a wait that has given the copies
@@ -583,6 +584,9 @@ __device__ void pa_many(const PrefixAttnParams& p, const PartJob& j, char* lds) 
     if (t0 + u < t1) issue(t0 + u, u);
   PaCols<DT, D, NB, NB == 1> w;
   pa_load_cols(p, j, j.col0 + wave * 16 * NB, lane, w);
+  // The queries are waited for here: left to their first use, the compiler would put its wait,
+  // which knows nothing of the copies, into the loop and drain them at every tile.
+  wait_vmcnt<0>();
   PaState<D, NB> st;
   pa_clear(st);
   int stage = 0;
