@@ -203,11 +203,14 @@ __device__ __forceinline__ float pa_max4(float v) {  // over lanes l, l ^ 16, l 
 }
 
 // A wave's running state over NB blocks of 16 columns: lane (g, l16) holds dims 16 db + 4 g ..
-// + 3 of column l16 of each block in o, and its own keys' part of the sum in l.
+// + 3 of column l16 of each block in o, and its own keys' part of the sum in l.  The exponents
+// are taken against m, which moves only for a score that lies past `limit` (2^8 times m's
+// exponential; any score while there is no m): the ratio of the sums is the same whatever m
+// is, and p <= 256 stays well inside the types.  neg = -m log2(e) scale, 0 while there is no m.
 template <int D, int NB>
 struct PaState {
   f32x4 o[D / 16][NB];
-  float m[NB], l[NB];
+  float m[NB], l[NB], limit[NB], neg[NB];
 };
 
 // A column's row, -1 for a padding column, PA_BLIND - row for one that sees nothing here.
@@ -219,6 +222,7 @@ template <int DT, int D, int NB, bool SCORES>
 struct PaCols {
   typename Mma<DT>::Frag q[NB][D / 32];
   int row[NB], first[NB], last[NB];
+  int all_first, all_last;          // keys within them every column sees
   float* score[SCORES ? NB : 1];  // this lane's column's scores (from key 0 on), or NULL
 };
 
@@ -247,6 +251,13 @@ __device__ __forceinline__ void pa_load_cols(const PrefixAttnParams& p, const Pa
                         ? p.score + (((int64_t)j.b * p.Hkv + j.hk) * j.cols + col) * p.spad
                         : nullptr;
   }
+  int lo = w.first[0], hi = w.last[0];
+#pragma unroll
+  for (int nb = 1; nb < NB; ++nb) lo = max(lo, w.first[nb]), hi = min(hi, w.last[nb]);
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) lo = max(lo, __shfl_xor(lo, o)), hi = min(hi, __shfl_xor(hi, o));
+  w.all_first = __builtin_amdgcn_readfirstlane(lo);
+  w.all_last = __builtin_amdgcn_readfirstlane(hi);
 }
 
 // A tile of KB * 16 keys from key0 on, in three steps.  Scores: S^T = K Q^T from the K rows in
@@ -276,11 +287,8 @@ __device__ __forceinline__ void pa_scores(const PaCols<DT, D, NB, SC>& w, const 
 template <int DT, int D, int NB, int KB, bool SC>
 __device__ __forceinline__ void pa_mask(const PaCols<DT, D, NB, SC>& w, f32x4 (&s)[KB][NB], int key0,
                                         int lane) {
+  if (key0 >= w.all_first && key0 + 16 * KB - 1 <= w.all_last) return;  // uniform
   const int g = lane >> 4;
-  bool edge = false;
-#pragma unroll
-  for (int nb = 0; nb < NB; ++nb) edge |= w.first[nb] > key0 || w.last[nb] < key0 + 16 * KB - 1;
-  if (!__ballot(edge)) return;
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
@@ -305,36 +313,43 @@ __device__ __forceinline__ void pa_keep(const PaCols<DT, D, NB, SC>& w, const f3
         *(f32x4*)(w.score[nb] + key0 + 16 * kb + 4 * (lane >> 4)) = s[kb][nb] * c;
 }
 
-// Turns masked scores into probabilities against the running maximum.
+// Turns masked scores into probabilities against the running reference, and sums them.
 template <int D, int NB, int KB>
 __device__ __forceinline__ void pa_softmax(PaState<D, NB>& st, f32x4 (&s)[KB][NB], float c) {
+  float mx[NB];  // of this lane's keys
+  bool past = false;
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
-    float mx = st.m[nb];
+    mx[nb] = s[0][nb][0];
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) mx = fmaxf(mx, s[kb][nb][e]);
-    mx = pa_max4(mx);
-    // The exponents' reference moves only past 2^8, or on the first finite score (the same
-    // ratio whatever it is; p <= 256 stays well inside the types).
-    const bool move = st.m[nb] == PA_NONE ? mx != PA_NONE : (mx - st.m[nb]) * c > 8.0f;
-    if (__ballot(move)) {
-      const float mnew = move ? mx : st.m[nb];
+      for (int e = 0; e < 4; ++e) mx[nb] = fmaxf(mx[nb], s[kb][nb][e]);
+    past |= mx[nb] > st.limit[nb];
+  }
+  if (__ballot(past)) {
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      const float top = pa_max4(mx[nb]);
+      if (!(top > st.limit[nb])) continue;
       const float alpha =
-          st.m[nb] == PA_NONE ? 0.0f : __builtin_amdgcn_exp2f((st.m[nb] - mnew) * c);
+          st.m[nb] == PA_NONE ? 0.0f : __builtin_amdgcn_exp2f((st.m[nb] - top) * c);
 #pragma unroll
       for (int db = 0; db < D / 16; ++db) st.o[db][nb] *= alpha;
       st.l[nb] *= alpha;
-      st.m[nb] = mnew;
+      st.m[nb] = top;
+      st.limit[nb] = top + 8.0f / c;
+      st.neg[nb] = -(top * c);
     }
-    const float msub = st.m[nb] == PA_NONE ? 0.0f : st.m[nb] * c;
+  }
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
     float sum = 0.0f;
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float pe = __builtin_amdgcn_exp2f(fmaf(s[kb][nb][e], c, -msub));
+        const float pe = __builtin_amdgcn_exp2f(fmaf(s[kb][nb][e], c, st.neg[nb]));
         s[kb][nb][e] = pe;
         sum += pe;
       }
@@ -391,8 +406,8 @@ template <int D, int NB>
 __device__ __forceinline__ void pa_clear(PaState<D, NB>& st) {
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
-    st.m[nb] = PA_NONE;
-    st.l[nb] = 0.0f;
+    st.m[nb] = st.limit[nb] = PA_NONE;
+    st.l[nb] = st.neg[nb] = 0.0f;
 #pragma unroll
     for (int db = 0; db < D / 16; ++db) st.o[db][nb] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
@@ -420,10 +435,15 @@ struct PaCopy {
                                         int lane) const {
     const int64_t off = (int64_t)key0 * stride;
     const bool whole = key0 >= lo && key0 + keys <= hi;  // uniform
+    if (whole) {
+#pragma unroll
+      for (int u = 0; u < N; ++u) async_copy16_to(src[u] + off, dst + u * 1024);
+      return;
+    }
 #pragma unroll
     for (int u = 0; u < N; ++u) {
       const uint16_t* s = src[u] + off;
-      if (!whole && (key0 + row[u] < lo || key0 + row[u] >= hi))
+      if (key0 + row[u] < lo || key0 + row[u] >= hi)
         s = (const uint16_t*)((const char*)g_zero_kib + lane * 16);
       async_copy16_to(s, dst + u * 1024);
     }
