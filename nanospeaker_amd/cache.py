@@ -6,7 +6,7 @@ with a cache; the reference decodes with one cache per sequence and evicts nothi
 
 Keys lie in the caches as attention multiplies them: normalised and rotated (`rotary_embed`,
 or the prefill, whose key heads `decoder.attn_prefill` leaves that way in its projection).
-Forward only.
+`DecodeCache` holds them for a decoder (`Decoder.prefix`, `Decoder.step`).  Forward only.
 """
 
 from __future__ import annotations
@@ -228,3 +228,87 @@ def _share(a: Tensor, b: Tensor) -> bool:
         return False
     (a0, a1), (b0, b1) = span(a), span(b)
     return a0 < b1 and b0 < a1
+
+
+class DecodeCache:
+    """
+    What a decoder keeps of a batch of sequences behind one prefix: the prefix's keys and values
+    of each layer once (prefix_kv, [P, key heads, dim]), each sequence's own (k, v [batch, rows,
+    key heads, dim]) with each layer's lengths (lens int32 [batch]), the accumulated weights of
+    the layers without a window (weights, or None), and the position of the next token
+    (positions int64 [batch]).  Made by Decoder.prefix, filled by Decoder.step.
+
+    `filled` bounds every length from above without asking the device; a step that would pass
+    the cache's rows is refused.
+    """
+
+    def __init__(self, windows, prefix_kv, prefix_len: int, batch: int, rows: int, n_kv_heads: int,
+                 dim: int, dtype, device, weights: bool = False):
+        n = len(windows)
+        if rows < 1 or batch < 1:
+            raise ValueError(f"DecodeCache: {batch} sequences of {rows} rows")
+        if prefix_len and len(prefix_kv) != n:
+            raise ValueError(f"DecodeCache: prefix of {len(prefix_kv)} layers for {n}")
+        self.windows, self.rows, self.batch, self.filled = list(windows), rows, batch, 0
+        self.prefix_kv = list(prefix_kv) if prefix_len else [(None, None)] * n
+        shape = (batch, rows, n_kv_heads, dim)
+        self.k = [torch.empty(shape, dtype=dtype, device=device) for _ in range(n)]
+        self.v = [torch.empty(shape, dtype=dtype, device=device) for _ in range(n)]
+        self.lens = [torch.zeros(batch, dtype=torch.int32, device=device) for _ in range(n)]
+        self.weights = [torch.zeros((batch, n_kv_heads, rows), dtype=torch.float32, device=device)
+                        if weights and w is None else None for w in windows]
+        self.positions = torch.full((batch,), prefix_len, dtype=torch.int64, device=device)
+        self._seq = torch.arange(batch, device=device)[:, None]
+
+    def reserve(self, idx: Tensor) -> None:
+        """Refuses tokens idx [batch, n] that the cache has no rows for."""
+        if idx.dim() != 2 or idx.shape[0] != self.batch or idx.shape[1] < 1:
+            raise ValueError(f"DecodeCache: tokens {tuple(idx.shape)}, expected [{self.batch}, n]")
+        if self.filled + idx.shape[1] > self.rows:
+            raise ValueError(f"DecodeCache: {idx.shape[1]} tokens more than the {self.rows} rows "
+                             f"hold ({self.filled} used)")
+
+    def next_positions(self, n: int) -> Tensor:
+        """The positions [batch, n] of the next n tokens."""
+        return self.positions[:, None] + torch.arange(n, device=self.positions.device)
+
+    def append(self, layer: int, k: Tensor, v: Tensor) -> None:
+        """Keys and values [batch, n, key heads, dim] behind a layer's rows."""
+        n = k.shape[1]
+        at = self.lens[layer][:, None] + torch.arange(n, device=k.device)
+        self.k[layer].index_put_((self._seq, at), k)
+        self.v[layer].index_put_((self._seq, at), v)
+        self.lens[layer] += n
+
+    def attend(self, layer: int, q: Tensor, window: "int | None") -> Tensor:
+        """Attention of the last tokens' q [batch, n, heads, dim] in a layer."""
+        w, lens, n = self.weights[layer], self.lens[layer], q.shape[1]
+        args = (*self.prefix_kv[layer], self.k[layer], self.v[layer])
+        if w is None:
+            return shared_prefix_attention(q, *args, lens, window=window)
+        # weights are accumulated over at most 64 queries a call: a prompt goes in pieces, each
+        # with the rows up to its own last token
+        m = max(1, 64 * w.shape[1] // q.shape[2])
+        o = [shared_prefix_attention(q[:, i:i + m], *args, lens - max(0, n - i - m), window=window,
+                                     weights=w, weights_out=w)[0] for i in range(0, n, m)]
+        return o[0] if len(o) == 1 else torch.cat(o, dim=1)
+
+    def advance(self, n: int) -> None:
+        self.positions += n
+        self.filled += n
+
+    def evict(self, budget: int, recent: int = 0, sinks: int = 0) -> None:
+        """Cuts the layers that accumulate weights down to `budget` rows a sequence (cache_evict).
+        Layers with a window keep all of theirs: a window counts rows."""
+        if all(w is None for w in self.weights):
+            raise ValueError("DecodeCache: nothing to evict by, made without weights")
+        for i, w in enumerate(self.weights):
+            if w is None:
+                continue
+            k, v = torch.empty_like(self.k[i]), torch.empty_like(self.v[i])
+            new = torch.zeros_like(w)
+            r = cache_evict(self.k[i], self.v[i], w, self.lens[i], budget, recent=recent,
+                            sinks=sinks, out=(k, v, new))
+            self.k[i], self.v[i], self.weights[i], self.lens[i] = k, v, new, r[4]
+        if all(w is not None for w in self.weights):
+            self.filled = min(self.filled, budget)

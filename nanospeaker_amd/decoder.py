@@ -37,9 +37,11 @@ import torch.nn.functional as F
 from torch import nn
 
 from . import _native as nat
+from .cache import DecodeCache
 from .head import linear_cross_entropy
 from .moe import MoEBlock
 from .moe_kernel import PACKS, PackCache, _stream
+from .rope import rotary_embed
 
 
 @dataclass
@@ -110,6 +112,17 @@ class Rotary:
                                 / self.d_head)
             ang = torch.arange(n, dtype=torch.float32, device=device)[:, None] * inv[None, :]
             hit = self._tables[key] = (ang.cos().to(dtype), ang.sin().to(dtype))
+        return hit
+
+    def freqs(self, device) -> torch.Tensor:
+        """The planes' frequencies for rotary_embed: the tables' fp32 ones, in fp64."""
+        key = ("freqs", str(device))
+        hit = self._tables.get(key)
+        if hit is None:
+            half = self.d_head // 2
+            inv = self.base ** (-torch.arange(half, dtype=torch.float32, device=device) * 2.0
+                                / self.d_head)
+            hit = self._tables[key] = inv.double()
         return hit
 
     def tables_f32(self, n: int, device):
@@ -340,31 +353,59 @@ class Attention(nn.Module):
             return x @ w
         return torch.addmm(resid, x, w) if out is None else out.addmm_(x, w)
 
-    def _kernel_attention(self, z: torch.Tensor) -> torch.Tensor:
-        """[B T, h dh]: the attention output before W_O, on the HIP prefill kernels."""
+    def _kernel_attention(self, z: torch.Tensor, keep: "list | None" = None) -> torch.Tensor:
+        """[B T, h dh]: the attention output before W_O, on the HIP prefill kernels.  With
+        `keep` the first sequence's keys (normalised and rotated) and values, [T, hk, dh] each,
+        are appended to it."""
         B, T, _ = z.shape
         qkv = self._project(z.reshape(B * T, -1), "qkv", (self.h + 2 * self.hk) * self.dh,
                             self.W_q, self.W_k, self.W_v)
         cos, sin = self.rotary.tables_f32(T, z.device)
-        return attn_prefill(qkv, B, T, self.h, self.hk, self.q_norm.gamma, self.k_norm.gamma,
-                            cos, sin, self.window, self.q_norm.eps)
+        o = attn_prefill(qkv, B, T, self.h, self.hk, self.q_norm.gamma, self.k_norm.gamma,
+                         cos, sin, self.window, self.q_norm.eps)
+        if keep is not None:
+            heads = qkv.view(B, T, self.h + 2 * self.hk, self.dh)[0, :, self.h:]
+            keep.append((heads[:, :self.hk].contiguous(), heads[:, self.hk:].contiguous()))
+        return o
 
-    def forward_residual(self, x: torch.Tensor, z: torch.Tensor,
-                         inplace: bool = False) -> torch.Tensor:
+    def decode(self, x: torch.Tensor, z: torch.Tensor, cache: DecodeCache,
+               layer: int) -> torch.Tensor:
+        """x + attention of the n new tokens z [B, n, d] over the cache's prefix and the
+        sequences' own rows, to which their keys and values are appended."""
+        if not self.use_kernel(z):
+            raise RuntimeError("Attention.decode: the kernel path only (gradient-free bf16 or fp16 "
+                               "on the GPU, 64-wide heads, 1-4 query heads per key/value head)")
+        B, n, d = z.shape
+        qkv = self._project(z.reshape(B * n, d), "qkv", (self.h + 2 * self.hk) * self.dh,
+                            self.W_q, self.W_k, self.W_v)
+        heads = qkv.view(B, n, self.h + 2 * self.hk, self.dh)
+        q, k = rotary_embed(self.q_norm(heads[:, :, :self.h]),
+                            self.k_norm(heads[:, :, self.h:self.h + self.hk]),
+                            cache.next_positions(n), self.rotary.freqs(z.device), inplace=True)
+        cache.append(layer, k, heads[:, :, self.h + self.hk:])
+        o = cache.attend(layer, q, self.window)
+        return self._project(o.view(B * n, self.h * self.dh), "o", d, self.W_O,
+                             resid=_as(x.reshape(B * n, d), x.dtype)).view(B, n, d)
+
+    def forward_residual(self, x: torch.Tensor, z: torch.Tensor, inplace: bool = False,
+                         keep: "list | None" = None) -> torch.Tensor:
         """x + self(z): on the kernel path the residual enters the W_O product as its addend
         (one rounding of x + o W_O instead of two); elsewhere exactly x + self(z).  With
         `inplace` (a caller that owns x and needs it no more) the kernel path accumulates
-        into x's own memory and returns x."""
+        into x's own memory and returns x.  `keep`: see _kernel_attention (kernel path only)."""
         if self.use_kernel(z) and x.dtype == z.dtype and not (
                 torch.is_grad_enabled() and x.requires_grad):
             B, T, d = x.shape
-            o = self._kernel_attention(z)
+            o = self._kernel_attention(z, keep)
             if inplace and x.is_contiguous():
                 xr = x.view(B * T, d)
                 self._project(o, "o", d, self.W_O, resid=xr, out=xr)
                 return x
             return self._project(o, "o", d, self.W_O,
                                  resid=_as(x.reshape(B * T, d), x.dtype)).view(B, T, d)
+        if keep is not None:
+            raise RuntimeError("Attention: keys and values are kept on the kernel path only (a "
+                               "gradient-free bf16 or fp16 forward on the GPU)")
         return x + self(z)
 
     def forward(self, z: torch.Tensor) -> torch.Tensor:
@@ -466,3 +507,33 @@ class Decoder(nn.Module):
         h = x[:, :-1].reshape(-1, self.cfg.d_model)
         y = targets[:, 1:].reshape(-1)
         return linear_cross_entropy(h, self.embed.weight, y), aux
+
+    @torch.no_grad()
+    def prefix(self, idx: torch.Tensor, batch: int, rows: int,
+               weights: bool = False) -> DecodeCache:
+        """A cache for `batch` sequences that all begin with the tokens idx [P] (P may be 0),
+        with room for `rows` more tokens each: the prefix is run once and its keys and values
+        kept once.  `weights`: the layers without a window also accumulate what attention gives
+        each cached row, for DecodeCache.evict.  bf16 or fp16 on the GPU, eval mode."""
+        kept: list = []
+        if idx.numel():
+            x = self.embed(idx.view(1, -1))
+            for blk in self.blocks:
+                x = blk.attn.forward_residual(x, blk.norm_attn(x), inplace=True, keep=kept)
+                x = blk.ffn.forward_residual(x, blk.norm_ffn)
+        c = self.cfg
+        w = self.embed.weight
+        return DecodeCache([c.layer_window(i) for i in range(c.n_layers)], kept, idx.numel(),
+                           batch, rows, c.n_kv_heads, c.d_head, w.dtype, w.device, weights)
+
+    @torch.no_grad()
+    def step(self, idx: torch.Tensor, cache: DecodeCache) -> torch.Tensor:
+        """Logits [B, n, vocab] of the next n tokens idx [B, n] of each of the cache's sequences,
+        which are appended to it."""
+        cache.reserve(idx)
+        x = self.embed(idx)
+        for i, blk in enumerate(self.blocks):
+            x = blk.attn.decode(x, blk.norm_attn(x), cache, i)
+            x = blk.ffn.forward_residual(x, blk.norm_ffn)
+        cache.advance(idx.shape[1])
+        return self.norm_out(x) @ self.embed.weight.t()
