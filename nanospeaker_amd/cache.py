@@ -28,6 +28,12 @@ def _fail(op: str, what: str):
     raise ValueError(f"{op}: {what}")
 
 
+def _forward_only(op: str, *tensors) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        _fail(op, "forward only: an operand requires a gradient (call it under torch.no_grad, or "
+                  "detach)")
+
+
 def _lens(op: str, lens: Tensor, b: int, device) -> None:
     if (lens.dtype is not torch.int32 or lens.shape != (b,) or lens.device != device
             or not lens.is_contiguous()):
@@ -114,6 +120,7 @@ def shared_prefix_attention(q: Tensor, k_prefix: Optional[Tensor], v_prefix: Opt
         _fail(op, "caches need a contiguous last dim, and strides and addresses that are multiples "
                   "of 16 bytes")
     _lens(op, lens, b, dev)
+    _forward_only(op, q, k, v, k_prefix, v_prefix, weights)
     if window is None:
         window = 0
     elif window < 1:
@@ -133,6 +140,9 @@ def shared_prefix_attention(q: Tensor, k_prefix: Optional[Tensor], v_prefix: Opt
             _fail(op, f"weights for at most 64 queries per key head, got {n * (hq // hk)}")
         if weights_out is None:
             weights_out = torch.empty_like(weights)
+        elif weights is not None and weights_out.data_ptr() != weights.data_ptr() and _share(
+                weights, weights_out):
+            _fail(op, "weights_out overlaps weights without being them")
     if b and n:
         a = nat.prefix_attn_args(
             _DT16[dt], d, hq, hk, b, n, p, s, min(int(window), (1 << 30) - 1),
@@ -176,6 +186,9 @@ def cache_evict(k: Tensor, v: Tensor, weights: Tensor, lens: Tensor, budget: int
                   f"got {k.dtype} {tuple(k.shape)} and {v.dtype} {tuple(v.shape)} on {k.device}")
     b, s, hk, d = k.shape
     dev = k.device
+    if hk < 1 or d < 1:
+        _fail(op, f"caches {tuple(k.shape)} without heads or dims")
+    _forward_only(op, k, v, weights)
     budget, recent, sinks = int(budget), int(recent), int(sinks)
     if budget < 1 or recent < 0 or sinks < 0 or recent + sinks > budget:
         _fail(op, f"budget {budget} with {sinks} sinks and {recent} recent rows")
@@ -207,7 +220,7 @@ def cache_evict(k: Tensor, v: Tensor, weights: Tensor, lens: Tensor, budget: int
             _fail(op, "the last dim must be contiguous")
     index = torch.empty((b, hk, budget), dtype=torch.int32, device=dev)
     lens_out = torch.empty_like(lens)
-    if b and hk and d:
+    if b:
         a = nat.evict_args(
             k.element_size(), hk, d, out is None, b, s, rows, budget, recent, sinks,
             k.data_ptr(), v.data_ptr(), k_out.data_ptr(), v_out.data_ptr(), *k.stride()[:3],

@@ -515,6 +515,8 @@ class Decoder(nn.Module):
         with room for `rows` more tokens each: the prefix is run once and its keys and values
         kept once.  `weights`: the layers without a window also accumulate what attention gives
         each cached row, for DecodeCache.evict.  bf16 or fp16 on the GPU, eval mode."""
+        if idx.dim() != 1:
+            raise ValueError(f"Decoder.prefix: tokens {tuple(idx.shape)}, expected [P]")
         kept: list = []
         if idx.numel():
             x = self.embed(idx.view(1, -1))

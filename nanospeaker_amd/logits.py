@@ -1,6 +1,6 @@
 """
 Between the head's logits and the choice of a token: penalties for repeated tokens, a bias and
-a grammar mask, in one pass of the library's kernel (nsmoe_penalize_logits).
+a grammar mask, in one pass of the library's kernel (nsmoe_penalize_logits).  Forward only.
 """
 
 from __future__ import annotations
@@ -59,6 +59,9 @@ def penalize_logits(logits: Tensor, history: Optional[Tensor] = None,
     if logits.dim() != 2 or not logits.is_cuda or logits.dtype not in _DT:
         raise ValueError("penalize_logits: logits must be a bf16, fp16 or fp32 [batch, vocab] GPU "
                          f"tensor, got {logits.dtype} {tuple(logits.shape)} on {logits.device}")
+    if logits.requires_grad and torch.is_grad_enabled():
+        raise ValueError("penalize_logits: forward only, and logits requires a gradient (call it "
+                         "under torch.no_grad, or detach)")
     b, v = logits.shape
     dev = logits.device
     if v > 1 and logits.stride(1) != 1:

@@ -81,6 +81,25 @@ def _writable(t: Tensor) -> bool:
     return True
 
 
+def _meet(a: Tensor, b: Tensor) -> bool:
+    """Whether the heads of two [batch, tokens, heads, dim] tensors share elements: column blocks
+    of one row are told apart, other views of common memory count as sharing."""
+    def span(t, dims):
+        return sum((t.shape[i] - 1) * t.stride(i) for i in dims) * t.element_size()
+    size = a.element_size()
+    pa, pb = a.data_ptr(), b.data_ptr()
+    if pa + span(a, range(4)) + size <= pb or pb + span(b, range(4)) + size <= pa:
+        return False
+    row_a, row_b = span(a, (2, 3)) + size, span(b, (2, 3)) + size
+    far = min((t.stride(i) * size for t in (a, b) for i in (0, 1) if t.shape[i] > 1),
+              default=None)
+    apart = pb - pa if pb >= pa else pa - pb
+    first = row_a if pb >= pa else row_b
+    rest = row_b if pb >= pa else row_a
+    same = all(a.stride(i) == b.stride(i) or a.shape[i] == 1 for i in (0, 1))
+    return not (same and apart >= first and (far is None or apart + rest <= far))
+
+
 _NO_STRIDES = (0, 0, 0)
 
 
@@ -180,8 +199,8 @@ def rotary_embed(q: Tensor, k: Optional[Tensor], positions: Tensor, freqs: Tenso
             if t is not None and t.numel() and (t.stride(3) != 1 or not _writable(t)):
                 raise ValueError("rotary_embed: inplace needs a contiguous last dim and elements "
                                  "that share no memory")
-        if k4 is not None and k4.numel() and k4.data_ptr() == q4.data_ptr():
-            raise ValueError("rotary_embed: inplace with q and k at one address")
+        if k4 is not None and k4.numel() and q4.numel() and _meet(q4, k4):
+            raise ValueError("rotary_embed: inplace with q and k that share elements")
         _launch(q4, k4, positions, freqs, interleaved, amplitude, False, True)
         return q, k
     if grad:

@@ -162,6 +162,7 @@ def test_captured_call_replays_with_new_inputs():
 
 def test_refusals():
     k, v, w, lens = make(2, 30, 2, 64)
+    one, flat = k.clone(), k[:1].clone().expand(2, 30, 2, 64)
     bad = [
         (dict(k=k.cpu()), "GPU"), (dict(k=k.double(), v=v.double()), "byte"),
         (dict(v=v[:, :20]), "one 2- or 4-byte"), (dict(v=v.half()), "one 2- or 4-byte"),
@@ -170,7 +171,10 @@ def test_refusals():
         (dict(budget=0), "budget"), (dict(budget=3, recent=2, sinks=2), "budget"),
         (dict(recent=-1), "budget"), (dict(k=k.transpose(2, 3), v=v.transpose(2, 3)), "weights"),
         (dict(k=k.transpose(2, 3).contiguous().transpose(2, 3)), "contiguous"),
-        (dict(out=(k, v, w)), "shares memory"),
+        (dict(out=(k, v, w)), "shares memory"), (dict(out=(one, one, w.clone())), "shares memory"),
+        (dict(out=(flat, v.clone(), w.clone())), "share memory"),
+        (dict(k=k[..., :0], v=v[..., :0]), "without"),
+        (dict(weights=w.clone().requires_grad_()), "forward only"),
         (dict(out=(k[:, :5].clone(), v[:, :5].clone(), w[..., :5].clone())), "out must"),
     ]
     for change, needle in bad:

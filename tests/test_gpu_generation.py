@@ -155,5 +155,7 @@ def test_refusals():
         plain.prefix(torch.arange(5, device=DEV), 2, rows=2)
     with pytest.raises(RuntimeError, match="kernel path"):
         plain.step(tok, plain.prefix(torch.arange(0, device=DEV), 2, rows=2))
+    with pytest.raises(ValueError, match="expected \\[P\\]"):
+        d.prefix(torch.zeros(1, 5, dtype=torch.int64, device=DEV), 2, rows=2)
     with pytest.raises(ValueError, match="0 rows"):
         d.prefix(torch.arange(5, device=DEV), 2, rows=0)

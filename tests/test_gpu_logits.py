@@ -214,6 +214,8 @@ def test_refusals():
         args = dict(kw, x=x) | change
         with pytest.raises(ValueError, match=needle):
             run(args.pop("x"), args)
+    with pytest.raises(ValueError, match="forward only"):
+        penalize_logits(x.clone().requires_grad_())
     with pytest.raises(ValueError, match="need a history"):
         penalize_logits(x, frequency=kw["frequency"])
     big = torch.zeros(2 * 100 + 8, device=DEV)

@@ -152,6 +152,32 @@ def test_against_64_bits(dtype, b, n, p, s, hq, hk, d, window):
     run(case, window, weights=w)
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("b", [1, 2, 4, 9])
+@pytest.mark.parametrize("n,g", [(5, 2), (5, 4), (10, 5), (20, 5), (25, 9)])
+def test_every_pair_of_forms(d, b, n, g):
+    """Own parts of 10, 20, 50, 100 and 225 columns beside prefix parts of one to nine times as
+    many, over lengths that end inside tiles, with a window that cuts both."""
+    print(f"[prefix] forms {(d, b, n, g)}", flush=True)
+    case = make(b, n, 150, 135, g, 1, d, torch.bfloat16, seed=b * n)
+    run(case)
+    run(case, window=140)
+
+
+@pytest.mark.parametrize("n,g", [(1, 3), (4, 3), (12, 4), (40, 5)])
+def test_rows_that_no_query_sees_may_hold_anything(n, g):
+    """NaN in every prefix and cache row before the oldest query's window."""
+    q, kp, vp, k, v, lens = make(3, n, 100, 90, g, 1, 64, torch.bfloat16, lens=[90, 77, 50])
+    k, v = clean(k), clean(v)
+    want = shared_prefix_attention(q, kp, vp, k, v, lens, window=8, return_lse=True)
+    for i, ln in enumerate((90, 77, 50)):
+        oldest = max(0, ln - n - 7)
+        k[i, :oldest], v[i, :oldest] = NAN, NAN
+    kp[:], vp[:] = NAN, NAN
+    got = shared_prefix_attention(q, kp, vp, k, v, lens, window=8, return_lse=True)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
 @pytest.mark.parametrize("lens", [[0, 0, 0], [1, 2, 3], [4, 3, 40], [-7, 41, 2 ** 31 - 1]])
 @pytest.mark.parametrize("n", [1, 4])
 @pytest.mark.parametrize("window", [None, 3])
@@ -328,6 +354,12 @@ def test_refusals():
         with pytest.raises(ValueError, match=needle):
             shared_prefix_attention(*[args.pop(n) for n in ("q", "k_prefix", "v_prefix", "k", "v",
                                                             "lens")], **args)
+    both = torch.zeros(2 * 60 + 8, device=DEV)
+    with pytest.raises(ValueError, match="overlaps"):
+        shared_prefix_attention(q, kp, vp, k, v, lens, weights=both[:120].view(2, 2, 30),
+                                weights_out=both[8:].view(2, 2, 30))
+    with pytest.raises(ValueError, match="forward only"):
+        shared_prefix_attention(q.clone().requires_grad_(), kp, vp, k, v, lens)
     big = make(1, 33, 5, 40, 2, 1, 64, torch.bfloat16)
     with pytest.raises(ValueError, match="at most 64"):
         shared_prefix_attention(*big, weights=torch.zeros(1, 1, 40, device=DEV))

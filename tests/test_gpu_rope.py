@@ -193,6 +193,69 @@ def test_second_derivative_is_the_rotation_again():
     check("double", back, *ref(v, pos, freqs, False, 1.0))
 
 
+def test_heads_that_share_memory_in_place():
+    """Column blocks of one row in either order, and blocks of separate tensors, are no overlap."""
+    freqs, _ = rotary_frequencies(64, device=DEV)
+    pos = torch.arange(5, device=DEV)
+    base = torch.randn(2, 5, 7, 64, device=DEV)
+    for q, k in ((slice(0, 4), slice(4, 7)), (slice(3, 7), slice(0, 3)), (slice(0, 2), slice(5, 7))):
+        x = base.clone()
+        want = rotary_embed(base[:, :, q], base[:, :, k], pos, freqs)
+        rotary_embed(x[:, :, q], x[:, :, k], pos, freqs, inplace=True)
+        assert torch.equal(x[:, :, q], want[0]) and torch.equal(x[:, :, k], want[1])
+
+
+def test_gradient_of_a_broadcast_operand():
+    """One key head expanded to four: its gradient is the sum over them (fp32; three additions
+    of values of at most |sum| of their sizes on top of the rotation's bound)."""
+    freqs, _ = rotary_frequencies(64, device=DEV)
+    pos = torch.arange(6, device=DEV)
+    leaf = torch.randn(2, 6, 1, 64, device=DEV, requires_grad=True)
+    y, _ = rotary_embed(leaf.expand(2, 6, 4, 64), None, pos, freqs)
+    g = torch.randn_like(y)
+    (got,) = torch.autograd.grad(y, leaf, g)
+    want, slack = ref(g, pos[None], freqs, False, 1.0, inverse=True)
+    size = want.abs().sum(2, keepdim=True)
+    check("leaf", got, want.sum(2, keepdim=True), slack.sum(2, keepdim=True) + 4 * 2.0 ** -24 * size)
+
+
+def test_captured_training_step():
+    """Forward and backward in one graph, replayed with new inputs between eager steps."""
+    freqs, amp = rotary_frequencies(32, 10_000.0, "yarn", 2.0, device=DEV)
+    pos = torch.arange(9, device=DEV)
+
+    def step(q, k, gq, gk):
+        yq, yk = rotary_embed(q, k, pos, freqs, amplitude=amp)
+        return (yq, yk, *torch.autograd.grad((yq, yk), (q, k), (gq, gk)))
+
+    def inputs(seed):
+        q, k, _ = make(2, 9, 3, 1, 64, torch.float32, seed=seed)
+        gq, gk, _ = make(2, 9, 3, 1, 64, torch.float32, seed=seed + 50)
+        return [q.detach().clone().requires_grad_(), k.detach().clone().requires_grad_(),
+                gq.clone(), gk.clone()]
+
+    held = inputs(0)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(*held)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(*held)
+    for seed in (1, 2, 3):
+        new = inputs(seed)
+        with torch.no_grad():
+            for a, b in zip(held, new):
+                a.copy_(b)
+        graph.replay()
+        want = step(*new)
+        torch.cuda.synchronize()
+        for a, b in zip(out, want):
+            assert torch.equal(a, b), seed
+
+
 def test_captured_call_replays_with_new_inputs():
     q, k, pos = make(3, 8, 9, 3, 64, torch.bfloat16)
     freqs, _ = rotary_frequencies(64, device=DEV)
@@ -214,6 +277,7 @@ def test_captured_call_replays_with_new_inputs():
 def test_refusals():
     q, k, pos = make(1, 4, 3, 1, 64, torch.bfloat16)
     freqs, _ = rotary_frequencies(64, device=DEV)
+    fused = torch.zeros(1, 4, 6, 64, dtype=torch.bfloat16, device=DEV)
     bad = [
         (dict(q=q.cpu()), "GPU"), (dict(q=q.double()), "bf16"), (dict(q=q[..., 0]), "does not go"),
         (dict(k=k.float()), "does not go"), (dict(k=k[:, :2]), "does not go"),
@@ -222,7 +286,9 @@ def test_refusals():
         (dict(freqs=torch.cat((freqs, freqs))), "rot_dim"), (dict(freqs=freqs[:0]), "rot_dim"),
         (dict(q=q.clone().requires_grad_(), inplace=True), "inplace"),
         (dict(q=q[:, :, :1].expand(1, 4, 3, 64), inplace=True), "inplace"),
-        (dict(k=q, inplace=True), "one address"),
+        (dict(k=q, inplace=True), "share elements"),
+        (dict(q=fused[:, :, :4], k=fused[:, :, 3:5], inplace=True), "share elements"),
+        (dict(q=fused[:, :, 3:5], k=fused[:, :, :4], inplace=True), "share elements"),
     ]
     for change, needle in bad:
         args = dict(q=q, k=k, positions=pos, freqs=freqs) | change
