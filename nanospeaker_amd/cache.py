@@ -18,7 +18,7 @@ import torch
 from torch import Tensor
 
 from . import _native as nat
-from .moe_kernel import _stream, on_device
+from .moe_kernel import call_on
 from .rope import _writable
 
 _DT16 = {torch.bfloat16: nat.BF16, torch.float16: nat.F16}
@@ -29,7 +29,7 @@ def _fail(op: str, what: str):
 
 
 def _forward_only(op: str, *tensors) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+    if torch.is_grad_enabled() and True in [t is not None and t.requires_grad for t in tensors]:
         _fail(op, "forward only: an operand requires a gradient (call it under torch.no_grad, or "
                   "detach)")
 
@@ -62,6 +62,13 @@ def _rows16(t: Tensor) -> "Optional[tuple[int, ...]]":
     if t.numel() == 0:
         return s
     return None if bits & 7 or t.stride(-1) != 1 or t.data_ptr() & 15 else s
+
+
+def _attend(a, dev, stream: int) -> None:
+    lib = nat.lib()
+    size = lib.nsmoe_prefix_attention_workspace_size(a)
+    ws = torch.empty(size, dtype=torch.uint8, device=dev)
+    nat.check(lib.nsmoe_prefix_attention(a, ws.data_ptr(), size, stream), "nsmoe_prefix_attention")
 
 
 def shared_prefix_attention(q: Tensor, k_prefix: Optional[Tensor], v_prefix: Optional[Tensor],
@@ -101,36 +108,47 @@ def shared_prefix_attention(q: Tensor, k_prefix: Optional[Tensor], v_prefix: Opt
     s, hk = k.shape[1], k.shape[2]
     if (k_prefix is None) != (v_prefix is None):
         _fail(op, "k_prefix without v_prefix, or v_prefix without k_prefix")
-    p = kp = vp = 0
-    skp = svp = (0, 0)
+    p = kp = vp = bits = 0
+    skp = svp = (0, 0, 1)
     if k_prefix is not None:
         if (k_prefix.dim() != 3 or k_prefix.shape != v_prefix.shape or k_prefix.shape[1] != hk
                 or k_prefix.shape[2] != d):
             _fail(op, f"prefix {tuple(k_prefix.shape)}, {tuple(v_prefix.shape)}, expected [rows, "
                       f"{hk}, {d}]")
+        if (k_prefix.dtype is not dt or v_prefix.dtype is not dt or k_prefix.device != dev
+                or v_prefix.device != dev):
+            _fail(op, f"the prefix has another type or device than q's {dt} on {dev}")
         p = k_prefix.shape[0]
         kp, vp = k_prefix.data_ptr(), v_prefix.data_ptr()
-        skp, svp = _rows16(k_prefix), _rows16(v_prefix)
-    for t in (k, v) if k_prefix is None else (k, v, k_prefix, v_prefix):
-        if t.dtype is not dt or t.device != dev:
-            _fail(op, f"a cache is {t.dtype} on {t.device}, another type or device than q's "
-                      f"{dt} on {dev}")
-    sk, sv = _rows16(k), _rows16(v)
-    if sk is None or sv is None or skp is None or svp is None:
-        _fail(op, "caches need a contiguous last dim, and strides and addresses that are multiples "
-                  "of 16 bytes")
+        skp, svp = k_prefix.stride(), v_prefix.stride()
+        bits = (kp | vp) >> 1 | skp[0] | skp[1] | svp[0] | svp[1]
+    if k.dtype is not dt or v.dtype is not dt or k.device != dev or v.device != dev:
+        _fail(op, f"a cache has another type or device than q's {dt} on {dev}")
+    sq, sk, sv = q.stride(), k.stride(), v.stride()
+    ka, va = k.data_ptr(), v.data_ptr()
+    bits |= ((ka | va | q.data_ptr()) >> 1 | sk[0] | sk[1] | sk[2] | sv[0] | sv[1] | sv[2] | sq[0]
+             | sq[1] | sq[2])
+    if bits & 7 or not sq[3] == sk[3] == sv[3] == skp[2] == svp[2] == 1:
+        # something is off 16 bytes, or only a stride that does not matter
+        sk, sv = _rows16(k), _rows16(v)
+        if p:
+            skp, svp = _rows16(k_prefix), _rows16(v_prefix)
+        if sk is None or sv is None or skp is None or svp is None:
+            _fail(op, "caches need a contiguous last dim, and strides and addresses that are "
+                      "multiples of 16 bytes")
+        sq = _rows16(q)
+        if sq is None:
+            q = q.clone(memory_format=torch.contiguous_format)
+            sq = q.stride()
     _lens(op, lens, b, dev)
-    _forward_only(op, q, k, v, k_prefix, v_prefix, weights)
+    if torch.is_grad_enabled():
+        _forward_only(op, q, k, v, k_prefix, v_prefix, weights)
     if window is None:
         window = 0
     elif window < 1:
         _fail(op, f"window {window}")
-    sq = _rows16(q)
-    if sq is None:
-        q = q.clone(memory_format=torch.contiguous_format)
-        sq = q.stride()[:-1]
     out = q.new_empty((b, n, hq, d))
-    lse = torch.empty((b, n, hq), dtype=torch.float32, device=dev) if return_lse else None
+    lse = q.new_empty((b, n, hq), dtype=torch.float32) if return_lse else None
     if weights is not None or weights_out is not None:
         for name, t in (("weights", weights), ("weights_out", weights_out)):
             if t is not None and (t.dtype is not torch.float32 or t.shape != (b, hk, s)
@@ -147,16 +165,11 @@ def shared_prefix_attention(q: Tensor, k_prefix: Optional[Tensor], v_prefix: Opt
         a = nat.prefix_attn_args(
             _DT16[dt], d, hq, hk, b, n, p, s, min(int(window), (1 << 30) - 1),
             1.0 / math.sqrt(d) if scale is None else float(scale), q.data_ptr(), kp, vp,
-            k.data_ptr(), v.data_ptr(), *sq, *skp, *svp, *sk, *sv, lens.data_ptr(),
+            ka, va, *sq[:3], *skp[:2], *svp[:2], *sk[:3], *sv[:3], lens.data_ptr(),
             out.data_ptr(), 0 if lse is None else lse.data_ptr(),
             0 if weights is None else weights.data_ptr(),
             0 if weights_out is None else weights_out.data_ptr())
-        lib = nat.lib()
-        with on_device(dev):
-            size = lib.nsmoe_prefix_attention_workspace_size(a)
-            ws = torch.empty(size, dtype=torch.uint8, device=dev)
-            nat.check(lib.nsmoe_prefix_attention(a, ws.data_ptr(), size, _stream(dev.index)),
-                      "nsmoe_prefix_attention")
+        call_on(dev, _attend, a, dev)
     elif weights_out is not None and weights_out is not weights:
         weights_out.zero_() if weights is None else weights_out.copy_(weights)
     if lse is None and weights_out is None:
@@ -227,8 +240,7 @@ def cache_evict(k: Tensor, v: Tensor, weights: Tensor, lens: Tensor, budget: int
             *v.stride()[:3], *k_out.stride()[:3], *v_out.stride()[:3], weights.data_ptr(),
             w_out.data_ptr(), *weights.stride()[:2], *w_out.stride()[:2], lens.data_ptr(),
             lens_out.data_ptr(), index.data_ptr())
-        with on_device(dev):
-            nat.check(nat.lib().nsmoe_cache_evict(a, _stream(dev.index)), "nsmoe_cache_evict")
+        nat.check(call_on(dev, nat.lib().nsmoe_cache_evict, a), "nsmoe_cache_evict")
     return k_out, v_out, w_out, index, lens_out
 
 

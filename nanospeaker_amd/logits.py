@@ -11,7 +11,7 @@ import torch
 from torch import Tensor
 
 from . import _native as nat
-from .moe_kernel import _DT, _stream, on_device
+from .moe_kernel import _DT, call_on
 
 
 def _vector(name: str, t: Optional[Tensor], n: int, dtype, device) -> int:
@@ -96,8 +96,7 @@ def penalize_logits(logits: Tensor, history: Optional[Tensor] = None,
         _vector("frequency", frequency, b, f32, dev), _vector("presence", presence, b, f32, dev),
         *((0, 0) if bias is None else _rows("bias", bias, b, v, f32, dev)),
         *((0, 0) if mask is None else _rows("mask", mask, b, (v + 31) // 32, i32, dev)))
-    with on_device(dev):
-        nat.check(nat.lib().nsmoe_penalize_logits(a, _stream(dev.index)), "nsmoe_penalize_logits")
+    nat.check(call_on(dev, nat.lib().nsmoe_penalize_logits, a), "nsmoe_penalize_logits")
     return out
 
 

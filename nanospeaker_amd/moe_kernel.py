@@ -101,15 +101,17 @@ def _stream(device_index: "int | None" = None) -> int:
     return _raw_stream(device_index)
 
 
-def on_device(device):
-    """A context in which `device` is the current one (nothing to do when it already is): a
-    launch goes to the current device, whatever device its stream belongs to."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return _HERE
-    return torch.cuda.device(device)
+_current_device = _private(torch._C, "_cuda_getDevice") or torch.cuda.current_device
 
 
-_HERE = nullcontext()
+def call_on(device, fn, *args):
+    """fn(*args, the device's current stream) with `device` the current one: a launch goes to
+    the current device, whatever device its stream belongs to."""
+    index = device.index
+    if index == _current_device():
+        return fn(*args, _stream(index))
+    with torch.cuda.device(device):
+        return fn(*args, _stream(index))
 
 
 def _p(t: Optional[Tensor]) -> Optional[int]:

@@ -21,7 +21,7 @@ import torch
 from torch import Tensor
 
 from . import _native as nat
-from .moe_kernel import _DT, _stream, on_device
+from .moe_kernel import _DT, call_on
 
 SCALINGS = (None, "linear", "ntk", "yarn")
 
@@ -127,8 +127,7 @@ def _launch(q: Optional[Tensor], k: Optional[Tensor], positions: Tensor, freqs: 
     a = nat.rope_args(_DT[some.dtype], interleaved, inverse, amplitude, b, n, hq, hk, d,
                       2 * freqs.shape[0], qp, kp, op, okp, *sq, *sk, *soq, *sok,
                       positions.data_ptr(), *positions.stride(), freqs.data_ptr())
-    with on_device(dev):
-        nat.check(nat.lib().nsmoe_rope(a, _stream(dev.index)), "nsmoe_rope")
+    nat.check(call_on(dev, nat.lib().nsmoe_rope, a), "nsmoe_rope")
     return oq, ok
 
 
@@ -189,7 +188,8 @@ def rotary_embed(q: Tensor, k: Optional[Tensor], positions: Tensor, freqs: Tenso
             2 <= 2 * freqs.shape[0] <= d):
         raise ValueError(f"rotary_embed: freqs must be fp64 [rot_dim / 2] on {q.device}, rot_dim "
                          f"2 .. {d}; got {freqs.dtype} {tuple(freqs.shape)} on {freqs.device}")
-    freqs = freqs.contiguous()
+    if freqs.stride(0) != 1:
+        freqs = freqs.contiguous()
     amplitude = float(amplitude)
     grad = torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))
     if inplace:

@@ -245,7 +245,10 @@ def test_strided_operands():
     odd = torch.zeros(q.numel() + 1, dtype=q.dtype, device=DEV)[1:].view(q.shape)
     odd.copy_(q)  # a query off the 16-byte alignment is copied
     third = shared_prefix_attention(odd, kp, vp, k, v, lens, return_lse=True)
-    for r in (got, other, third):
+    every = torch.zeros(3, 2, 9, 64 * 9, dtype=q.dtype, device=DEV)[..., ::9]
+    every.copy_(q)  # and one whose last dim is strided
+    fourth = shared_prefix_attention(every, kp, vp, k, v, lens, return_lse=True)
+    for r in (got, other, third, fourth):
         assert torch.equal(r[0], want[0]) and torch.equal(r[1], want[1])
 
 
@@ -348,6 +351,8 @@ def test_refusals():
         (dict(weights=w[..., :20]), "weights"), (dict(weights_out=w.transpose(0, 1)), "weights"),
         (dict(k=torch.zeros(k.numel() + 1, dtype=q.dtype, device=DEV)[1:].view(k.shape)), "16 bytes"),
         (dict(k=k.transpose(2, 3).contiguous().transpose(2, 3)), "16 bytes"),
+        (dict(v=torch.zeros(2, 30, 2, 64 * 9, dtype=q.dtype, device=DEV)[..., ::9]), "16 bytes"),
+        (dict(k_prefix=torch.zeros(20, 2, 64 * 17, dtype=q.dtype, device=DEV)[..., ::17]), "16 bytes"),
     ]
     for change, needle in bad:
         args = dict(q=q, k_prefix=kp, v_prefix=vp, k=k, v=v, lens=lens) | change
