@@ -24,8 +24,9 @@ namespace nsmoe {
 
 constexpr int LG_NT = 512;
 constexpr int LG_VEC = 8;           // logits per thread and step: one byte of mask
-constexpr int LG_MAX_SLICE = 16384;  // 64 KiB of table: two workgroups per CU
+constexpr int LG_MAX_SLICE = 8192;   // 32 KiB of table: four workgroups per CU
 constexpr int LG_MIN_SLICE = 1024;
+constexpr int LG_IDS = 8;            // history loads of a thread in flight
 
 struct LogitParams {
   const void* x;
@@ -65,10 +66,18 @@ __global__ void __launch_bounds__(LG_NT) logits_kernel(LogitParams p) {
     n = n < 0 ? 0 : n > p.L ? p.L : n;
     const int64_t np = p.prompt ? p.prompt[b] : 0;
     const int64_t* h = p.hist + b * p.ldh;
-    for (int64_t j = tid; j < n; j += LG_NT) {
-      const uint64_t at = (uint64_t)h[j] - (uint64_t)v0;
-      if (at < (uint64_t)nv) {
-        if (j < np) atomicOr(&s_tab[at], 0x80000000u);
+    for (int64_t j0 = tid; j0 < n; j0 += LG_IDS * LG_NT) {
+      int64_t id[LG_IDS];
+#pragma unroll
+      for (int u = 0; u < LG_IDS; ++u) {
+        const int64_t j = j0 + u * LG_NT;
+        id[u] = j < n ? h[j] : -1;
+      }
+#pragma unroll
+      for (int u = 0; u < LG_IDS; ++u) {
+        const uint64_t at = (uint64_t)id[u] - (uint64_t)v0;
+        if (id[u] < 0 || at >= (uint64_t)nv) continue;
+        if (j0 + u * LG_NT < np) atomicOr(&s_tab[at], 0x80000000u);
         else atomicAdd(&s_tab[at], 1u);
       }
     }
@@ -93,34 +102,50 @@ __global__ void __launch_bounds__(LG_NT) logits_kernel(LogitParams p) {
     v += bv;
     return allowed ? v : -INFINITY;
   };
-  for (int i = tid * LG_VEC; i < nv; i += LG_NT * LG_VEC) {
-    uint32_t w[LG_VEC] = {};
-    if constexpr (HIST) {
-      const u32x4 a = *(const u32x4*)(s_tab + i), c = *(const u32x4*)(s_tab + i + 4);
+  // Two steps' loads are issued before the first one's store, which may be to the same memory
+  // and holds later loads back.
+  constexpr int U = 2;
+  for (int i0 = tid * LG_VEC; i0 < nv; i0 += U * LG_NT * LG_VEC) {
+    Run8<TI> in[U];
+    Run8<float> bv[U] = {};
+    uint32_t bits[U];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) w[e] = a[e], w[4 + e] = c[e];
+    for (int k = 0; k < U; ++k) {
+      const int i = i0 + k * LG_NT * LG_VEC;
+      bits[k] = mask && i < nv ? mask[i / 8] : 0xffu;
+      if (i + LG_VEC <= nv) {
+        in[k] = *(const Run8<TI>*)(x + i);
+        if (bias) bv[k] = *(const Run8<float>*)(bias + i);
+      }
     }
-    const uint32_t bits = mask ? mask[i / 8] : 0xffu;
-    if (i + LG_VEC <= nv) {
-      const Run8<TI> in = *(const Run8<TI>*)(x + i);
-      Run8<float> bv = {};
-      if (bias) bv = *(const Run8<float>*)(bias + i);
-      float o[LG_VEC];
 #pragma unroll
-      for (int e = 0; e < LG_VEC; ++e)
-        o[e] = change(Elem<DT>::to_f(in.e[e]), w[e], bias ? bv.e[e] : 0.0f, (bits >> e) & 1);
-      TO r[LG_VEC];
-      round_to<ODT>(o, r);
-      Run8<TO> out;
+    for (int k = 0; k < U; ++k) {
+      const int i = i0 + k * LG_NT * LG_VEC;
+      if (i >= nv) break;
+      uint32_t w[LG_VEC] = {};
+      if constexpr (HIST) {
+        const u32x4 a = *(const u32x4*)(s_tab + i), c = *(const u32x4*)(s_tab + i + 4);
 #pragma unroll
-      for (int e = 0; e < LG_VEC; ++e) out.e[e] = r[e];
-      *(Run8<TO>*)(y + i) = out;
-    } else {
+        for (int e = 0; e < 4; ++e) w[e] = a[e], w[4 + e] = c[e];
+      }
+      if (i + LG_VEC <= nv) {
+        float o[LG_VEC];
 #pragma unroll
-      for (int e = 0; e < LG_VEC; ++e)
-        if (i + e < nv)
-          y[i + e] = Elem<ODT>::from_f(change(Elem<DT>::to_f(x[i + e]), w[e],
-                                              bias ? bias[i + e] : 0.0f, (bits >> e) & 1));
+        for (int e = 0; e < LG_VEC; ++e)
+          o[e] = change(Elem<DT>::to_f(in[k].e[e]), w[e], bv[k].e[e], (bits[k] >> e) & 1);
+        TO r[LG_VEC];
+        round_to<ODT>(o, r);
+        Run8<TO> out;
+#pragma unroll
+        for (int e = 0; e < LG_VEC; ++e) out.e[e] = r[e];
+        *(Run8<TO>*)(y + i) = out;
+      } else {
+#pragma unroll
+        for (int e = 0; e < LG_VEC; ++e)
+          if (i + e < nv)
+            y[i + e] = Elem<ODT>::from_f(change(Elem<DT>::to_f(x[i + e]), w[e],
+                                                bias ? bias[i + e] : 0.0f, (bits[k] >> e) & 1));
+      }
     }
   }
 }

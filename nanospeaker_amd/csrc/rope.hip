@@ -23,6 +23,7 @@
 namespace nsmoe {
 
 constexpr int RP_NT = 256;
+constexpr int RP_BATCH = 4;         // items of a thread in flight
 constexpr int RP_MAX_TOK = 16;      // tokens per workgroup
 constexpr int RP_MAX_TRIG = 1024;   // planes x tokens held in LDS, 8 bytes each
 
@@ -105,48 +106,63 @@ __global__ void __launch_bounds__(RP_NT) rope_kernel(RopeParams p) {
   constexpr int TV = IL && WIDE ? 2 * VP : VP;
   const int nrot = half / VP;
   const int n_items = ntok * (int)p.by_tok.d;
-  for (int i = threadIdx.x; i < n_items; i += RP_NT) {
-    const int t = (int)p.by_tok.div(i), u = i - t * (int)p.by_tok.d;
-    int h = (int)p.by_head.div(u);
-    const int c = u - h * (int)p.by_head.d;
-    const bool is_k = h >= p.nq;
-    if (is_k) h -= p.nq;
-    const char* src = is_k ? p.k.src + s_at[t][2] + h * p.k.sh : p.q.src + s_at[t][0] + h * p.q.sh;
-    char* dst = is_k ? p.k.dst + s_at[t][3] + h * p.k.dh : p.q.dst + s_at[t][1] + h * p.q.dh;
-    if (c >= nrot) {
-      const int64_t off = (int64_t)(p.rot + (c - nrot) * TV) * ES;
-      rope_store<DT, TV, WIDE>(dst + off, rope_load<DT, TV, WIDE>(src + off), p.stream);
-      continue;
-    }
-    const float* cs = s_cos + t * half + c * VP;
-    const float* sn = s_sin + t * half + c * VP;
-    if constexpr (IL) {
-      const int64_t off = (int64_t)c * 2 * VP * ES;
-      RopeVec<DT, 2 * VP> v = rope_load<DT, 2 * VP, WIDE>(src + off);
-      float o[2 * VP];
+  // RP_BATCH items' loads are issued before the first one's store (a store to what may be the
+  // same memory holds later loads back): 32 KiB in flight a CU do not cover HBM's latency.
+  using First = RopeVec<DT, IL ? 2 * VP : VP>;
+  for (int i0 = threadIdx.x; i0 < n_items; i0 += RP_BATCH * RP_NT) {
+    First va[RP_BATCH];
+    RopeVec<DT, VP> vb[RP_BATCH];  // the other half's planes
+    char* dst[RP_BATCH];
+    int trig[RP_BATCH];  // where the item's planes begin in the tables, -1: a tail vector
 #pragma unroll
-      for (int e = 0; e < VP; ++e) {
-        const float a = Elem<DT>::to_f(v.e[2 * e]), bb = Elem<DT>::to_f(v.e[2 * e + 1]);
-        o[2 * e] = a * cs[e] - bb * sn[e];
-        o[2 * e + 1] = bb * cs[e] + a * sn[e];
+    for (int k = 0; k < RP_BATCH; ++k) {
+      const int i = min(i0 + k * RP_NT, n_items - 1);
+      const int t = (int)p.by_tok.div(i), u = i - t * (int)p.by_tok.d;
+      int h = (int)p.by_head.div(u);
+      const int c = u - h * (int)p.by_head.d;
+      const bool is_k = h >= p.nq;
+      if (is_k) h -= p.nq;
+      const char* src =
+          is_k ? p.k.src + s_at[t][2] + h * p.k.sh : p.q.src + s_at[t][0] + h * p.q.sh;
+      dst[k] = is_k ? p.k.dst + s_at[t][3] + h * p.k.dh : p.q.dst + s_at[t][1] + h * p.q.dh;
+      trig[k] = c < nrot ? t * half + c * VP : -1;
+      const int64_t off = (int64_t)(c < nrot ? c * (IL ? 2 * VP : VP) : p.rot + (c - nrot) * TV) * ES;
+      dst[k] += off;
+      if (VP == 1 && IL && c >= nrot) va[k].e[0] = rope_load<DT, 1, WIDE>(src + off).e[0];
+      else va[k] = rope_load<DT, IL ? 2 * VP : VP, WIDE>(src + off);
+      if (!IL && c < nrot) vb[k] = rope_load<DT, VP, WIDE>(src + off + (int64_t)half * ES);
+    }
+#pragma unroll
+    for (int k = 0; k < RP_BATCH; ++k) {
+      if (i0 + k * RP_NT >= n_items) break;
+      if (trig[k] < 0) {
+        RopeVec<DT, TV> v;
+#pragma unroll
+        for (int e = 0; e < TV; ++e) v.e[e] = va[k].e[e];
+        rope_store<DT, TV, WIDE>(dst[k], v, p.stream);
+        continue;
       }
-      round_to<DT>(o, v.e);
-      rope_store<DT, 2 * VP, WIDE>(dst + off, v, p.stream);
-    } else {
-      const int64_t lo = (int64_t)c * VP * ES, hi = lo + (int64_t)half * ES;
-      RopeVec<DT, VP> va = rope_load<DT, VP, WIDE>(src + lo);
-      RopeVec<DT, VP> vb = rope_load<DT, VP, WIDE>(src + hi);
+      const float *cs = s_cos + trig[k], *sn = s_sin + trig[k];
       float oa[VP], ob[VP];
 #pragma unroll
       for (int e = 0; e < VP; ++e) {
-        const float a = Elem<DT>::to_f(va.e[e]), bb = Elem<DT>::to_f(vb.e[e]);
-        oa[e] = a * cs[e] - bb * sn[e];
-        ob[e] = bb * cs[e] + a * sn[e];
+        const float x1 = Elem<DT>::to_f(va[k].e[IL ? 2 * e : e]);
+        const float x2 = Elem<DT>::to_f(IL ? va[k].e[IL ? 2 * e + 1 : e] : vb[k].e[e]);
+        oa[e] = x1 * cs[e] - x2 * sn[e];
+        ob[e] = x2 * cs[e] + x1 * sn[e];
       }
-      round_to<DT>(oa, va.e);
-      round_to<DT>(ob, vb.e);
-      rope_store<DT, VP, WIDE>(dst + lo, va, p.stream);
-      rope_store<DT, VP, WIDE>(dst + hi, vb, p.stream);
+      if constexpr (IL) {
+        float o[2 * VP];
+#pragma unroll
+        for (int e = 0; e < VP; ++e) o[2 * e] = oa[e], o[2 * e + 1] = ob[e];
+        round_to<DT>(o, va[k].e);
+        rope_store<DT, 2 * VP, WIDE>(dst[k], va[k], p.stream);
+      } else {
+        round_to<DT>(oa, va[k].e);
+        round_to<DT>(ob, vb[k].e);
+        rope_store<DT, VP, WIDE>(dst[k], va[k], p.stream);
+        rope_store<DT, VP, WIDE>(dst[k] + (int64_t)half * ES, vb[k], p.stream);
+      }
     }
   }
 }
