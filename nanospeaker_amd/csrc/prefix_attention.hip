@@ -67,6 +67,22 @@ __device__ __forceinline__ int pa_len(const PrefixAttnParams& p, int b) {
   return n < 0 ? 0 : n > p.S ? p.S : n;
 }
 
+// The sequence with the r-th longest cache (the earlier one first among equals), for up to 64
+// sequences: the longest parts then start first, and the launch does not end on one that
+// started late (64 ragged sequences of 256 to 1024 rows, dim 128: 39 us against 42 unordered).
+// Lane l holds sequence l's length; the r-th largest is found bit by bit.
+__device__ __forceinline__ int pa_by_length(const PrefixAttnParams& p, int r) {
+  const int lane = threadIdx.x & 63;
+  const int len = lane < p.B ? pa_len(p, lane) : -1;
+  int v = 0;  // the largest value that more than r lengths reach
+  for (int bit = 1 << (31 - __clz(p.S | 1)); bit; bit >>= 1)
+    if (__popcll(__ballot(len >= v + bit)) > r) v += bit;
+  const int k = r - (int)__popcll(__ballot(len > v));  // which of the equal ones
+  const uint64_t same = __ballot(len == v);
+  const bool me = len == v && (int)__popcll(same & (((uint64_t)1 << lane) - 1)) == k;
+  return (int)__ffsll((unsigned long long)__ballot(me)) - 1;
+}
+
 // One part: a key/value head's columns against a run of keys.
 struct PartJob {
   const uint16_t *k, *v;  // the head's row 0
@@ -106,14 +122,19 @@ __device__ __forceinline__ PartJob pa_job(const PrefixAttnParams& p, int item, b
     item /= p.rbs;
     j.b = item % p.B;
     const int split = item / p.B;
+    if (p.B > 1 && p.B <= 64) j.b = pa_by_length(p, j.b);
     j.k = p.k + j.b * p.kb + j.hk * p.kh;
     j.v = p.v + j.b * p.vb + j.hk * p.vh;
     j.kt = p.kt;
     j.vt = p.vt;
     j.col0 = rb * width;
     j.cols = p.n * p.G;
-    j.key0 = split * p.chunk_s;
-    j.key1 = j.key0 + p.chunk_s;
+    // As many parts as the length is nearest to, of one size: a short remainder would pay a
+    // part's start and end for little (640 rows at 512 a part: 37 us in one, 40 in two).
+    const int len = pa_len(p, j.b), parts = max(1, (len + p.chunk_s / 2) / p.chunk_s);
+    const int size = ((len + parts - 1) / parts + 127) / 128 * 128;
+    j.key0 = split * size;
+    j.key1 = split < parts ? j.key0 + size : j.key0;
     j.slot = p.np + split;
   }
   return j;
