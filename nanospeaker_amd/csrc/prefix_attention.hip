@@ -58,13 +58,20 @@ struct PrefixAttnParams {
   int chunk_p, chunk_s;  // keys per part
   int rbp, rbs;          // column blocks of a prefix part and of an own part
   int items_p;           // workgroups of the prefix (before the own ones)
-  LaunchDiv by_G, by_n;
+  LaunchDiv by_G, by_n, by_seq, by_chunk;  // group's heads, new tokens, a sequence's rows, keys
   float scale_log2;
 };
 
 __device__ __forceinline__ int pa_len(const PrefixAttnParams& p, int b) {
   const int n = p.lens[b];
   return n < 0 ? 0 : n > p.S ? p.S : n;
+}
+
+// How many parts a sequence's own rows make: as many as the length is nearest to, of one size,
+// because a short remainder would pay a part's start and end for little.  The parts from there
+// to ns are not computed, and prefix_join_kernel does not look at them.
+__device__ __forceinline__ int pa_parts_of(const PrefixAttnParams& p, int len) {
+  return max(1, (int)p.by_chunk.div((uint32_t)(len + p.chunk_s / 2)));
 }
 
 // The sequence with the r-th longest cache (the earlier one first among equals), for up to 64
@@ -90,7 +97,7 @@ struct PartJob {
   int hk, b;              // b < 0: the prefix
   int col0, cols;         // first column, and how many columns there are in all
   int key0, key1;         // the part's keys
-  int slot;
+  int slot;               // -1: a part that this sequence does not have
 };
 
 __device__ __forceinline__ PartJob pa_job(const PrefixAttnParams& p, int item, bool own,
@@ -129,13 +136,12 @@ __device__ __forceinline__ PartJob pa_job(const PrefixAttnParams& p, int item, b
     j.vt = p.vt;
     j.col0 = rb * width;
     j.cols = p.n * p.G;
-    // As many parts as the length is nearest to, of one size: a short remainder would pay a
-    // part's start and end for little (640 rows at 512 a part: 37 us in one, 40 in two).
-    const int len = pa_len(p, j.b), parts = max(1, (len + p.chunk_s / 2) / p.chunk_s);
-    const int size = ((len + parts - 1) / parts + 127) / 128 * 128;
+    const int len = pa_len(p, j.b), parts = pa_parts_of(p, len);
+    // ceil(tiles / parts): exact, the quotient of two integers below 2^23 rounded once
+    const int size = (int)((float)((len + 127) / 128 + parts - 1) / (float)parts) * 128;
     j.key0 = split * size;
-    j.key1 = split < parts ? j.key0 + size : j.key0;
-    j.slot = p.np + split;
+    j.key1 = j.key0 + size;
+    j.slot = split < parts ? p.np + split : -1;
   }
   return j;
 }
@@ -674,6 +680,7 @@ constexpr int PA_WIDTH[PA_FORMS] = {16, 32, 64, 128, 192};
 template <int DT, int D, int FORM>
 __device__ __forceinline__ void pa_part(const PrefixAttnParams& p, int item, bool own, char* lds) {
   const PartJob j = pa_job(p, item, own, PA_WIDTH[FORM]);
+  if (j.slot < 0) return;
   if constexpr (FORM < 2) pa_few<DT, D, FORM + 1>(p, j, lds);
   else pa_many<DT, D, FORM - 1>(p, j, lds);
 }
@@ -706,7 +713,14 @@ __device__ __forceinline__ PaTotal pa_total(const PrefixAttnParams& p, int64_t r
   const int slots = p.np + p.ns;
   const float2* ml = p.part_ml + row * slots;
   const float2 none = make_float2(PA_NONE, 0.0f);
-  const float2 a = lane < slots ? ml[lane] : none, b = lane + 64 < slots ? ml[lane + 64] : none;
+  float2 a = lane < slots ? ml[lane] : none, b = lane + 64 < slots ? ml[lane + 64] : none;
+  // Slots of parts that the sequence does not have were not written: read (beside the length)
+  // and dropped.
+  if (p.ns > 1) {
+    const int live = p.np + pa_parts_of(p, pa_len(p, (int)p.by_seq.div((uint32_t)row)));
+    if (lane >= live) a = none;
+    if (lane + 64 >= live) b = none;
+  }
   PaTotal r;
   r.m = fmaxf(a.x, b.x);
   for (int o = 32; o; o >>= 1) r.m = fmaxf(r.m, __shfl_xor(r.m, o));
@@ -856,11 +870,13 @@ static PrefixPlan pa_plan(const nsmoe_prefix_attn_args* a) {
     pl.items_p = pl.np * groups;
   }
   if (pl.form_s >= 0) {
-    // Two parts a slot even ragged lengths out; a part's start and end cost about 2 us, so
-    // more lose (64 x 640 rows, dim 128: 37 us, 35 with one part, 40 with four).
+    // About 768 keys a part, or fewer while that leaves slots empty: a part's start and end cost
+    // about 2 us of its slot, and larger ones leave ragged lengths uneven (48 sequences of up to
+    // 8191 rows, dim 64, with weights: 52 us; 55 at 1024 keys, 57 at 1280.  32 x 2048 rows, dim
+    // 128: 44 us; 46 at 1024 and at 512).
     pl.rbs = (int)cdiv(n * G, PA_WIDTH[pl.form_s]);
     const int64_t groups = B * pl.rbs * a->n_kv_heads;
-    pl.chunk_s = chunk_of(a->cap, 2 * slots / groups);
+    pl.chunk_s = chunk_of(a->cap, std::max(cdiv(a->cap, 768), slots / groups));
     pl.ns = (int)cdiv(a->cap, pl.chunk_s);
     pl.items_s = pl.ns * groups;
   }
@@ -1034,6 +1050,8 @@ extern "C" int nsmoe_prefix_attention(const nsmoe_prefix_attn_args* a, void* wor
   P.items_p = (int)pl.items_p;
   P.by_G = launch_div(P.G);
   P.by_n = launch_div(P.n);
+  P.by_seq = launch_div((int64_t)P.n * P.Hq);
+  P.by_chunk = launch_div(P.chunk_s > 0 ? P.chunk_s : 1);
   P.scale_log2 = a->scale * 1.4426950408889634f;
   hipStream_t s = (hipStream_t)stream;
   if (a->head_dim == 64)
