@@ -16,6 +16,7 @@ from typing import Optional
 
 import torch
 from torch import Tensor
+from torch.autograd.graph import increment_version
 
 from . import _native as nat
 from .moe_kernel import call_on
@@ -142,7 +143,7 @@ def shared_prefix_attention(q: Tensor, k_prefix: Optional[Tensor], v_prefix: Opt
             sq = q.stride()
     _lens(op, lens, b, dev)
     if torch.is_grad_enabled():
-        _forward_only(op, q, k, v, k_prefix, v_prefix, weights)
+        _forward_only(op, q, k, v, k_prefix, v_prefix, weights, weights_out)
     if window is None:
         window = 0
     elif window < 1:
@@ -170,6 +171,8 @@ def shared_prefix_attention(q: Tensor, k_prefix: Optional[Tensor], v_prefix: Opt
             0 if weights is None else weights.data_ptr(),
             0 if weights_out is None else weights_out.data_ptr())
         call_on(dev, _attend, a, dev)
+        if weights_out is not None:
+            increment_version(weights_out)
     elif weights_out is not None and weights_out is not weights:
         weights_out.zero_() if weights is None else weights_out.copy_(weights)
     if lse is None and weights_out is None:
@@ -178,7 +181,8 @@ def shared_prefix_attention(q: Tensor, k_prefix: Optional[Tensor], v_prefix: Opt
 
 
 def cache_evict(k: Tensor, v: Tensor, weights: Tensor, lens: Tensor, budget: int, *,
-                recent: int = 0, sinks: int = 0, out: "tuple[Tensor, Tensor, Tensor] | None" = None):
+                recent: int = 0, sinks: int = 0,
+                out: "tuple[Tensor, Tensor, Tensor] | None" = None):
     """
     The caches k, v [batch, rows, key heads, dim] cut down to `budget` rows a sequence.  Of a
     sequence with more (lens[b], int32), each key head keeps its first `sinks` rows, its last
@@ -201,7 +205,7 @@ def cache_evict(k: Tensor, v: Tensor, weights: Tensor, lens: Tensor, budget: int
     dev = k.device
     if hk < 1 or d < 1:
         _fail(op, f"caches {tuple(k.shape)} without heads or dims")
-    _forward_only(op, k, v, weights)
+    _forward_only(op, k, v, weights, *(out or ()))
     budget, recent, sinks = int(budget), int(recent), int(sinks)
     if budget < 1 or recent < 0 or sinks < 0 or recent + sinks > budget:
         _fail(op, f"budget {budget} with {sinks} sinks and {recent} recent rows")
@@ -241,6 +245,8 @@ def cache_evict(k: Tensor, v: Tensor, weights: Tensor, lens: Tensor, budget: int
             w_out.data_ptr(), *weights.stride()[:2], *w_out.stride()[:2], lens.data_ptr(),
             lens_out.data_ptr(), index.data_ptr())
         nat.check(call_on(dev, nat.lib().nsmoe_cache_evict, a), "nsmoe_cache_evict")
+        if out is not None:
+            increment_version(out)
     return k_out, v_out, w_out, index, lens_out
 
 
@@ -264,7 +270,8 @@ class DecodeCache:
     (positions int64 [batch]).  Made by Decoder.prefix, filled by Decoder.step.
 
     `filled` bounds every length from above without asking the device; a step that would pass
-    the cache's rows is refused.
+    the cache's rows is refused.  So are steps under graph capture, whose replays this count
+    would miss, and steps after one that raised part way, which left its rows in some layers.
     """
 
     def __init__(self, windows, prefix_kv, prefix_len: int, batch: int, rows: int, n_kv_heads: int,
@@ -275,6 +282,7 @@ class DecodeCache:
         if prefix_len and len(prefix_kv) != n:
             raise ValueError(f"DecodeCache: prefix of {len(prefix_kv)} layers for {n}")
         self.windows, self.rows, self.batch, self.filled = list(windows), rows, batch, 0
+        self._open = False  # a step has written rows and not come to its end
         self.prefix_kv = list(prefix_kv) if prefix_len else [(None, None)] * n
         shape = (batch, rows, n_kv_heads, dim)
         self.k = [torch.empty(shape, dtype=dtype, device=device) for _ in range(n)]
@@ -286,12 +294,18 @@ class DecodeCache:
         self._seq = torch.arange(batch, device=device)[:, None]
 
     def reserve(self, idx: Tensor) -> None:
-        """Refuses tokens idx [batch, n] that the cache has no rows for."""
+        """Refuses a step of tokens idx [batch, n] that the cache cannot hold or count."""
         if idx.dim() != 2 or idx.shape[0] != self.batch or idx.shape[1] < 1:
             raise ValueError(f"DecodeCache: tokens {tuple(idx.shape)}, expected [{self.batch}, n]")
         if self.filled + idx.shape[1] > self.rows:
             raise ValueError(f"DecodeCache: {idx.shape[1]} tokens more than the {self.rows} rows "
                              f"hold ({self.filled} used)")
+        if self._open:
+            raise RuntimeError("DecodeCache: a step raised before its end and left its rows in "
+                               "some layers; make the cache anew")
+        if self.positions.is_cuda and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("DecodeCache: a step under graph capture (its replays would not "
+                               "count the rows they fill)")
 
     def next_positions(self, n: int) -> Tensor:
         """The positions [batch, n] of the next n tokens."""
@@ -300,6 +314,7 @@ class DecodeCache:
     def append(self, layer: int, k: Tensor, v: Tensor) -> None:
         """Keys and values [batch, n, key heads, dim] behind a layer's rows."""
         n = k.shape[1]
+        self._open = True
         at = self.lens[layer][:, None] + torch.arange(n, device=k.device)
         self.k[layer].index_put_((self._seq, at), k)
         self.v[layer].index_put_((self._seq, at), v)
@@ -314,13 +329,16 @@ class DecodeCache:
         # weights are accumulated over at most 64 queries a call: a prompt goes in pieces, each
         # with the rows up to its own last token
         m = max(1, 64 * w.shape[1] // q.shape[2])
-        o = [shared_prefix_attention(q[:, i:i + m], *args, lens - max(0, n - i - m), window=window,
+        o = [shared_prefix_attention(q[:, i:i + m], *args,
+                                     lens - (n - i - m) if i + m < n else lens, window=window,
                                      weights=w, weights_out=w)[0] for i in range(0, n, m)]
         return o[0] if len(o) == 1 else torch.cat(o, dim=1)
 
     def advance(self, n: int) -> None:
+        """Ends the step of n tokens."""
         self.positions += n
         self.filled += n
+        self._open = False
 
     def evict(self, budget: int, recent: int = 0, sinks: int = 0) -> None:
         """Cuts the layers that accumulate weights down to `budget` rows a sequence (cache_evict).
@@ -334,6 +352,8 @@ class DecodeCache:
             new = torch.zeros_like(w)
             r = cache_evict(self.k[i], self.v[i], w, self.lens[i], budget, recent=recent,
                             sinks=sinks, out=(k, v, new))
+            for t in (self.k[i], self.v[i], w, self.lens[i]):
+                t.record_stream(torch.cuda.current_stream(t.device))  # it may be of another
             self.k[i], self.v[i], self.weights[i], self.lens[i] = k, v, new, r[4]
         if all(w is not None for w in self.weights):
             self.filled = min(self.filled, budget)

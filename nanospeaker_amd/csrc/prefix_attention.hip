@@ -484,9 +484,8 @@ __device__ __forceinline__ uint32_t pa_lds(const char* p) {
   return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)p;
 }
 
-constexpr int FEW_KEYS_OF(int D) { return 32; }
 template <int D> struct PaGeo {
-  static constexpr int FEW_KEYS = FEW_KEYS_OF(D);
+  static constexpr int FEW_KEYS = 32;
   static constexpr int FEW_TILE = FEW_KEYS * 2 * D;  // bytes of K or V
   static constexpr int FEW_LDS = 4 * 2 * FEW_TILE;   // 32 or 64 KiB
   static constexpr int MANY_KEYS = 64;

@@ -9,6 +9,7 @@ from typing import Optional
 
 import torch
 from torch import Tensor
+from torch.autograd.graph import increment_version
 
 from . import _native as nat
 from .moe_kernel import _DT, call_on
@@ -59,11 +60,13 @@ def penalize_logits(logits: Tensor, history: Optional[Tensor] = None,
     if logits.dim() != 2 or not logits.is_cuda or logits.dtype not in _DT:
         raise ValueError("penalize_logits: logits must be a bf16, fp16 or fp32 [batch, vocab] GPU "
                          f"tensor, got {logits.dtype} {tuple(logits.shape)} on {logits.device}")
-    if logits.requires_grad and torch.is_grad_enabled():
-        raise ValueError("penalize_logits: forward only, and logits requires a gradient (call it "
-                         "under torch.no_grad, or detach)")
+    if torch.is_grad_enabled() and (logits.requires_grad
+                                    or (out is not None and out.requires_grad)):
+        raise ValueError("penalize_logits: forward only, and logits or out requires a gradient "
+                         "(call it under torch.no_grad, or detach)")
     b, v = logits.shape
     dev = logits.device
+    given = out
     if v > 1 and logits.stride(1) != 1:
         raise ValueError("penalize_logits: the rows of logits must be contiguous")
     if out is None:
@@ -97,6 +100,8 @@ def penalize_logits(logits: Tensor, history: Optional[Tensor] = None,
         *((0, 0) if bias is None else _rows("bias", bias, b, v, f32, dev)),
         *((0, 0) if mask is None else _rows("mask", mask, b, (v + 31) // 32, i32, dev)))
     nat.check(call_on(dev, nat.lib().nsmoe_penalize_logits, a), "nsmoe_penalize_logits")
+    if given is not None:
+        increment_version(given)
     return out
 
 

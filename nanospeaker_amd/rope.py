@@ -19,6 +19,7 @@ from typing import Optional
 
 import torch
 from torch import Tensor
+from torch.autograd.graph import increment_version
 
 from . import _native as nat
 from .moe_kernel import _DT, call_on
@@ -144,6 +145,8 @@ class _Rotate(torch.autograd.Function):
     @staticmethod
     def backward(ctx, gq, gk):
         dq = dk = None
+        gq = gq if ctx.needs_input_grad[0] else None
+        gk = gk if ctx.needs_input_grad[1] else None
         if gq is not None or gk is not None:
             interleaved, amplitude, inverse = ctx.how
             dq, dk = _Rotate.apply(gq, gk, *ctx.saved_tensors, interleaved, amplitude,
@@ -202,6 +205,7 @@ def rotary_embed(q: Tensor, k: Optional[Tensor], positions: Tensor, freqs: Tenso
         if k4 is not None and k4.numel() and q4.numel() and _meet(q4, k4):
             raise ValueError("rotary_embed: inplace with q and k that share elements")
         _launch(q4, k4, positions, freqs, interleaved, amplitude, False, True)
+        increment_version(q if k is None else (q, k))
         return q, k
     if grad:
         yq, yk = _Rotate.apply(q4, k4, positions, freqs, interleaved, amplitude, False)

@@ -16,7 +16,8 @@ import torch
 pytestmark = pytest.mark.gpu
 
 pytest.importorskip("nanospeaker_amd.moe_kernel")
-from nanospeaker_amd import penalize_logits  # noqa: E402
+from nanospeaker_amd import (cache_evict, penalize_logits, rotary_embed,  # noqa: E402
+                             rotary_frequencies, shared_prefix_attention)
 from nanospeaker_amd.decoder import Decoder, DecoderConfig  # noqa: E402
 
 DEV = "cuda"
@@ -159,3 +160,64 @@ def test_refusals():
         d.prefix(torch.zeros(1, 5, dtype=torch.int64, device=DEV), 2, rows=2)
     with pytest.raises(ValueError, match="0 rows"):
         d.prefix(torch.arange(5, device=DEV), 2, rows=0)
+
+
+def test_a_captured_step_is_refused():
+    d, _ = decoders(torch.bfloat16, layers=1)
+    cache = d.prefix(torch.arange(4, device=DEV), 2, 8)
+    idx = torch.zeros(2, 1, dtype=torch.int64, device=DEV)
+    d.step(idx, cache)
+    g = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="capture"):
+        with torch.cuda.graph(g):
+            cache.reserve(idx)
+    d.step(idx, cache)
+    assert cache.filled == 2
+
+
+def test_written_operands_are_known_to_autograd():
+    """What a call writes into its operands counts as an in-place change: a backward that saved
+    the old values raises rather than use the new ones."""
+    leaf = torch.randn(1, 3, 2, 64, device=DEV, requires_grad=True)
+    lens = torch.full((1,), 3, dtype=torch.int32, device=DEV)
+    freqs, _ = rotary_frequencies(64, device=DEV)
+    pos = torch.arange(3, device=DEV)[None]
+
+    def turn(t):
+        rotary_embed(t, None, pos, freqs, inplace=True)
+
+    def penalize(t):
+        penalize_logits(t[0, 0], out=t[0, 0])
+
+    def attend(t):
+        kv = torch.randn(1, 64, 2, 64, device=DEV, dtype=torch.bfloat16)
+        shared_prefix_attention(kv[:, :3], None, None, kv, kv, lens,
+                                weights_out=t.view(-1)[:128].view(1, 2, 64))
+
+    def evict(t):
+        kv = torch.randn(1, 3, 2, 64, device=DEV)
+        cache_evict(kv, kv, torch.zeros(1, 2, 3, device=DEV), lens, 2,
+                    out=(t, torch.empty_like(kv), torch.empty(1, 2, 3, device=DEV)))
+
+    for write in (turn, penalize, attend, evict):
+        print(f"[generation] {write.__name__}", flush=True)
+        saved = leaf * 1.0
+        loss = (saved * saved).sum()
+        write(saved.detach())
+        with pytest.raises(RuntimeError, match="inplace"):
+            loss.backward()
+
+
+def test_outputs_that_want_a_gradient_are_refused():
+    x = torch.zeros(2, 8, device=DEV)
+    with pytest.raises(ValueError, match="gradient"):
+        penalize_logits(x, out=torch.zeros_like(x).requires_grad_())
+    kv = torch.zeros(1, 4, 1, 64, device=DEV, dtype=torch.bfloat16)
+    lens = torch.full((1,), 4, dtype=torch.int32, device=DEV)
+    w = torch.zeros(1, 1, 4, device=DEV)
+    with pytest.raises(ValueError, match="gradient"):
+        shared_prefix_attention(kv[:, :1], None, None, kv, kv, lens,
+                                weights_out=torch.zeros_like(w).requires_grad_())
+    with pytest.raises(ValueError, match="gradient"):
+        cache_evict(kv, kv, w, lens, 2, out=(torch.zeros_like(kv).requires_grad_(),
+                                             torch.zeros_like(kv), torch.zeros_like(w)))
