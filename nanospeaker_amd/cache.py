@@ -68,8 +68,9 @@ def _rows16(t: Tensor) -> "Optional[tuple[int, ...]]":
 def _attend(a, dev, stream: int) -> None:
     lib = nat.lib()
     size = lib.nsmoe_prefix_attention_workspace_size(a)
-    ws = torch.empty(size, dtype=torch.uint8, device=dev)
-    nat.check(lib.nsmoe_prefix_attention(a, ws.data_ptr(), size, stream), "nsmoe_prefix_attention")
+    ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+    nat.check(lib.nsmoe_prefix_attention(a, None if ws is None else ws.data_ptr(), size, stream),
+              "nsmoe_prefix_attention")
 
 
 def shared_prefix_attention(q: Tensor, k_prefix: Optional[Tensor], v_prefix: Optional[Tensor],

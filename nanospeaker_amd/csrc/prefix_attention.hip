@@ -13,7 +13,8 @@
 // columns of one product, and the prefix is read once instead of batch times.  The own rows
 // are read by their sequence's columns alone.  Both are split over the keys into parts; a part
 // leaves its columns' running maximum, sum and unnormalised output in fp32, and
-// prefix_join_kernel joins them.
+// prefix_join_kernel joins them.  A decode step's short context takes one launch instead
+// (prefix_whole_kernel), each sequence's columns over the prefix and its own rows.
 //
 // Two forms of a part, by the number of columns:
 //   few   up to 32 columns (a decode step's own rows, or the prefix of a small batch): each
@@ -256,6 +257,18 @@ struct PaCols {
   float* score[SCORES ? NB : 1];  // this lane's column's scores (from key 0 on), or NULL
 };
 
+// The keys that every column of a wave sees.
+template <int DT, int D, int NB, bool SC>
+__device__ __forceinline__ void pa_common(PaCols<DT, D, NB, SC>& w) {
+  int lo = w.first[0], hi = w.last[0];
+#pragma unroll
+  for (int nb = 1; nb < NB; ++nb) lo = max(lo, w.first[nb]), hi = min(hi, w.last[nb]);
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) lo = max(lo, __shfl_xor(lo, o)), hi = min(hi, __shfl_xor(hi, o));
+  w.all_first = __builtin_amdgcn_readfirstlane(lo);
+  w.all_last = __builtin_amdgcn_readfirstlane(hi);
+}
+
 template <int DT, int D, int NB, bool SC>
 __device__ __forceinline__ void pa_load_cols(const PrefixAttnParams& p, const PartJob& j, int c0,
                                              int lane, PaCols<DT, D, NB, SC>& w) {
@@ -281,13 +294,7 @@ __device__ __forceinline__ void pa_load_cols(const PrefixAttnParams& p, const Pa
                         ? p.score + (((int64_t)j.b * p.Hkv + j.hk) * j.cols + col) * p.spad
                         : nullptr;
   }
-  int lo = w.first[0], hi = w.last[0];
-#pragma unroll
-  for (int nb = 1; nb < NB; ++nb) lo = max(lo, w.first[nb]), hi = min(hi, w.last[nb]);
-#pragma unroll
-  for (int o = 1; o < 16; o <<= 1) lo = max(lo, __shfl_xor(lo, o)), hi = min(hi, __shfl_xor(hi, o));
-  w.all_first = __builtin_amdgcn_readfirstlane(lo);
-  w.all_last = __builtin_amdgcn_readfirstlane(hi);
+  pa_common(w);
 }
 
 // A tile of KB * 16 keys from key0 on, in three steps.  Scores: S^T = K Q^T from the K rows in
@@ -313,11 +320,12 @@ __device__ __forceinline__ void pa_scores(const PaCols<DT, D, NB, SC>& w, const 
     }
 }
 
-// Keys outside a column's range: one select per score, on tiles that cross some edge only.
+// Keys outside a column's range, or past `top`: one select per score, on tiles that cross some
+// edge only.
 template <int DT, int D, int NB, int KB, bool SC>
 __device__ __forceinline__ void pa_mask(const PaCols<DT, D, NB, SC>& w, f32x4 (&s)[KB][NB], int key0,
-                                        int lane) {
-  if (key0 >= w.all_first && key0 + 16 * KB - 1 <= w.all_last) return;  // uniform
+                                        int lane, int top = INT32_MAX) {
+  if (key0 >= w.all_first && key0 + 16 * KB - 1 <= min(w.all_last, top)) return;  // uniform
   const int g = lane >> 4;
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb)
@@ -326,7 +334,7 @@ __device__ __forceinline__ void pa_mask(const PaCols<DT, D, NB, SC>& w, f32x4 (&
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int key = key0 + 16 * kb + 4 * g + e;
-        const bool dead = (key < w.first[nb]) | (key > w.last[nb]);
+        const bool dead = (key < w.first[nb]) | (key > min(w.last[nb], top));
         s[kb][nb][e] = dead ? PA_NONE : s[kb][nb][e];
       }
 }
@@ -494,6 +502,59 @@ template <int D> struct PaGeo {
   static constexpr int MANY_LDS = MANY_STAGES * 2 * MANY_TILE;  // 48 or 64 KiB
 };
 
+// Joins NW waves through their buffers, 16 columns at a time, and calls
+// emit(row, dim, maximum, sum, four dims of the output) for each column: the maximum is -inf for
+// one that saw nothing.
+template <int DT, int D, int NB, int NW, bool SC, class F>
+__device__ __forceinline__ void pa_join_waves(const PrefixAttnParams& p,
+                                              const PaCols<DT, D, NB, SC>& w,
+                                              const PaState<D, NB>& st, char* lds, F&& emit) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15, g = lane >> 4;
+  float* s_o = (float*)lds;                      // [NW][16][D]
+  float* s_m = (float*)(lds + NW * 16 * D * 4);  // [NW][16]
+  float* s_l = s_m + NW * 16;                    // [NW][16]
+  int* s_row = (int*)(s_l + NW * 16);            // [16]
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+    float l = st.l[nb];
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    __syncthreads();
+    if (g == 0) {
+      s_m[wave * 16 + l16] = st.m[nb];
+      s_l[wave * 16 + l16] = l;
+      s_row[l16] = w.row[nb];
+    }
+#pragma unroll
+    for (int db = 0; db < D / 16; ++db)
+      *(f32x4*)(s_o + (wave * 16 + l16) * D + 16 * db + 4 * g) = st.o[db][nb];
+    __syncthreads();
+    for (int i = threadIdx.x; i < 16 * (D / 4); i += NW * 64) {
+      const int col = i / (D / 4), d = (i % (D / 4)) * 4;
+      const int r = s_row[col], row = r <= PA_BLIND ? PA_BLIND - r : r;
+      if (row < 0) continue;
+      float m = PA_NONE;
+      if (r >= 0) {
+#pragma unroll
+        for (int k = 0; k < NW; ++k) m = fmaxf(m, s_m[k * 16 + col]);
+      }
+      f32x4 o = {0.f, 0.f, 0.f, 0.f};
+      float sum = 0.0f;
+      if (m != PA_NONE) {
+#pragma unroll
+        for (int k = 0; k < NW; ++k) {
+          const float mk = s_m[k * 16 + col];
+          if (mk == PA_NONE) continue;
+          const float f = __builtin_amdgcn_exp2f((mk - m) * p.scale_log2);
+          sum += s_l[k * 16 + col] * f;
+          o += *(const f32x4*)(s_o + (k * 16 + col) * D + d) * f;
+        }
+      }
+      emit(row, d, m, sum, o);
+    }
+  }
+}
+
 template <int DT, int D, int NB>
 __device__ void pa_few(const PrefixAttnParams& p, const PartJob& j, char* lds) {
   using Geo = PaGeo<D>;
@@ -558,53 +619,13 @@ __device__ void pa_few(const PrefixAttnParams& p, const PartJob& j, char* lds) {
 
   if (keep && raw_at >= 0) pa_keep(w, raw, raw_at, p.scale_log2, lane);
 
-  // Join the four waves through LDS, 16 columns at a time.
-  float* s_o = (float*)lds;                     // [4][16][D]
-  float* s_m = (float*)(lds + 4 * 16 * D * 4);  // [4][16]
-  float* s_l = s_m + 4 * 16;                    // [4][16]
-  int* s_row = (int*)(s_l + 4 * 16);            // [16]
-  const int slots = p.np + p.ns;
-#pragma unroll
-  for (int nb = 0; nb < NB; ++nb) {
-    float l = st.l[nb];
-    l += __shfl_xor(l, 16);
-    l += __shfl_xor(l, 32);
-    __syncthreads();
-    if (g == 0) {
-      s_m[wave * 16 + l16] = st.m[nb];
-      s_l[wave * 16 + l16] = l;
-      s_row[l16] = w.row[nb];
-    }
-#pragma unroll
-    for (int db = 0; db < D / 16; ++db)
-      *(f32x4*)(s_o + (wave * 16 + l16) * D + 16 * db + 4 * g) = st.o[db][nb];
-    __syncthreads();
-    for (int i = threadIdx.x; i < 16 * (D / 4); i += PA_NT) {
-      const int col = i / (D / 4), d = (i % (D / 4)) * 4;
-      const int r = s_row[col], row = r <= PA_BLIND ? PA_BLIND - r : r;
-      if (row < 0) continue;
-      float m = PA_NONE;
-      if (r >= 0) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) m = fmaxf(m, s_m[k * 16 + col]);
-      }
-      const int64_t at = (int64_t)row * slots + j.slot;
-      f32x4 o = {0.f, 0.f, 0.f, 0.f};
-      float sum = 0.0f;
-      if (m != PA_NONE) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float mk = s_m[k * 16 + col];
-          if (mk == PA_NONE) continue;
-          const float f = __builtin_amdgcn_exp2f((mk - m) * p.scale_log2);
-          sum += s_l[k * 16 + col] * f;
-          o += *(const f32x4*)(s_o + (k * 16 + col) * D + d) * f;
-        }
-        *(f32x4*)(p.part_o + at * D + d) = o;
-      }
-      if (d == 0) p.part_ml[at] = make_float2(m * p.scale_log2, sum);
-    }
-  }
+  const int64_t slots = p.np + p.ns;
+  pa_join_waves<DT, D, NB, 4>(p, w, st, lds, [&](int row, int d, float m, float sum,
+                                                const f32x4& o) {
+    const int64_t at = row * slots + j.slot;
+    if (m != PA_NONE) *(f32x4*)(p.part_o + at * D + d) = o;
+    if (d == 0) p.part_ml[at] = make_float2(m * p.scale_log2, sum);
+  });
 }
 
 template <int DT, int D, int NB>
@@ -673,6 +694,96 @@ __device__ void pa_many(const PrefixAttnParams& p, const PartJob& j, char* lds) 
 #pragma unroll
     for (int db = 0; db < D / 16; ++db) *(f32x4*)(dst + 16 * db) = st.o[db][nb];
   }
+}
+
+// A short context in one launch, without parts: a workgroup takes the columns, up to 16 NB, of
+// one sequence and key/value head over the prefix and then its own rows, its eight waves the
+// 32-key tiles of both in turn as in pa_few, and writes the output.  Keys are numbered through:
+// own row r is key P + r, and a column sees one run of them.  Bound by latency: a launch, the
+// lengths, the queries and a round of tiles after the other.  Eight waves take half the rounds of
+// four (512 + 1024 keys, dim 64: 9.6 us against 11.8) and fill 64 or 128 KiB of LDS.
+constexpr int PA_WHOLE_WAVES = 8;
+
+template <int DT, int D, int NB>
+__global__ void __launch_bounds__(PA_WHOLE_WAVES * 64, 2) prefix_whole_kernel(PrefixAttnParams p) {
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
+  using Geo = PaGeo<D>;
+  constexpr int KEYS = Geo::FEW_KEYS, TILE = Geo::FEW_TILE, KB = KEYS / 16;
+  constexpr int NC = TILE / 1024, NW = PA_WHOLE_WAVES;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  PartJob j{};
+  j.hk = (int)blockIdx.x % p.Hkv;
+  j.b = (int)blockIdx.x / p.Hkv;
+  j.cols = p.n * p.G;
+  j.key1 = p.S;
+  int lo, hi;  // own rows that some column sees
+  pa_range(p, j, 16 * NB, lane, lo, hi);
+  const int at0 = max(0, pa_len(p, j.b) - p.n);  // the first query's row
+  const int lo_p = p.window ? min(p.P, max(0, p.P + at0 - p.window + 1)) : 0;
+  const int tp0 = lo_p / KEYS, ts0 = lo / KEYS;
+  const int tp = hi > lo ? (p.P + KEYS - 1) / KEYS - tp0 : 0;
+  const int tiles = hi > lo ? tp + (hi + KEYS - 1) / KEYS - ts0 : 0;
+  const uint16_t *kp = p.kp + j.hk * p.kph, *vp = p.vp + j.hk * p.vph;
+  const uint16_t *ko = p.k + j.b * p.kb + j.hk * p.kh, *vo = p.v + j.b * p.vb + j.hk * p.vh;
+  char* Kt = lds + wave * 2 * TILE;
+  char* Vt = Kt + TILE;
+  const uint32_t kd = pa_lds(Kt), vd = kd + TILE;
+  auto copy = [&](int i, const uint16_t* prefix, int64_t prefix_rows, const uint16_t* cache,
+                  int64_t cache_rows, uint32_t dst) {
+    PaCopy<D, NC> c;
+    const bool own = i >= tp;
+    c.set(own ? cache : prefix, own ? cache_rows : prefix_rows, 0, lane);
+    const int tile = own ? ts0 + i - tp : tp0 + i;
+    c.issue(tile * KEYS, KEYS, own ? lo : lo_p, own ? hi : p.P, dst, lane);
+  };
+  auto copy_k = [&](int i) { copy(i, kp, p.kpt, ko, p.kt, kd); };
+  auto copy_v = [&](int i) { copy(i, vp, p.vpt, vo, p.vt, vd); };
+  int t = wave;
+  if (t < tiles) {
+    copy_k(t);
+    copy_v(t);
+  }
+  PaCols<DT, D, NB, false> w;
+  pa_load_cols(p, j, 0, lane, w);
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb)
+    if (w.row[nb] >= 0) {  // its own rows so far
+      w.first[nb] = p.window ? p.P + w.last[nb] - p.window + 1 : 0;
+      w.last[nb] += p.P;
+    }
+  pa_common(w);
+  wait_vmcnt<0>();  // see pa_many
+  PaState<D, NB> st;
+  pa_clear(st);
+  for (; t < tiles; t += NW) {
+    f32x4 s[KB][NB];
+    wait_vmcnt<NC>();  // this tile's K; its V stays in flight
+    asm volatile("" ::: "memory");
+    pa_scores(w, Kt, lane, s);
+    asm volatile("" ::: "memory");
+    wait_lgkm0();      // K has been read
+    const bool more = t + NW < tiles;
+    if (more) copy_k(t + NW);
+    if (t < tp) pa_mask(w, s, (tp0 + t) * KEYS, lane, p.P - 1);
+    else pa_mask(w, s, p.P + (ts0 + t - tp) * KEYS, lane);
+    pa_softmax(st, s, p.scale_log2);
+    if (more) wait_vmcnt<NC>();  // this tile's V; the next K stays in flight
+    else wait_vmcnt<0>();
+    asm volatile("" ::: "memory");
+    pa_values<DT, D, NB, KB, DT == DT_BF16>(st, s, Vt, lane);
+    asm volatile("" ::: "memory");
+    wait_lgkm0();      // V has been read
+    if (more) copy_v(t + NW);
+  }
+  pa_join_waves<DT, D, NB, NW>(p, w, st, lds, [&](int row, int d, float m, float sum, f32x4 o) {
+    if (m != PA_NONE) o *= 1.0f / sum;
+    *(uint2*)(p.out + (int64_t)row * D + d) =
+        make_uint2(pack2<DT>(o[0], o[1]), pack2<DT>(o[2], o[3]));
+    if (p.lse && d == 0)
+      p.lse[row] = m == PA_NONE ? PA_NONE
+                                : (m * p.scale_log2 + log2f(sum)) * 0.69314718055994531f;
+  });
 }
 
 // Forms: 0, 1 few with 1 or 2 column blocks; 2, 3, 4 many with 1, 2 or 3 per wave.
@@ -823,6 +934,7 @@ __global__ void __launch_bounds__(PA_NT) prefix_join_kernel(PrefixAttnParams p, 
 // ---- host -------------------------------------------------------------------------------
 
 struct PrefixPlan {
+  bool whole;          // no parts: prefix_whole_kernel
   int form_p, form_s;  // -1: no such parts
   int np, ns, chunk_p, chunk_s, rbp, rbs, spad;
   int64_t items_p, items_s, rows;
@@ -842,6 +954,17 @@ static PrefixPlan pa_plan(const nsmoe_prefix_attn_args* a) {
   const int64_t G = a->n_heads / a->n_kv_heads, B = a->batch, n = a->n_new, D = a->head_dim;
   const int64_t cus = device_cus(), slots = 2 * cus;  // workgroups that run at once
   pl.rows = B * n * a->n_heads;
+  // A short context is not split: up to 1536 keys of 64 dims or 768 of 128 that a sequence sees,
+  // while every workgroup has its CU (or half of one, at 64) at once.  4 sequences of 512 + 64
+  // keys, dim 64: 7.2 us in a graph and 11.3 called eagerly against 8.7 and 15.2 in parts, 64 of
+  // 512 + 1024 12.4 and 12.3 against 14.6 and 16.1; a single one of 2048 + 256 12.8 against 9.1.
+  const int64_t all = a->prefix_len + a->cap;
+  const int64_t seen = a->window ? std::min<int64_t>(all, a->window + n - 1) : all;
+  if (a->cap > 0 && n * G <= 32 && !a->weights_out && seen * D <= 1536 * 64 &&
+      B * a->n_kv_heads * D <= slots * 64) {
+    pl.whole = true;
+    return pl;
+  }
   pl.form_p = a->prefix_len > 0 ? pa_form(B * n * G, a->head_dim) : -1;
   pl.form_s = a->cap > 0 ? pa_form(n * G, a->head_dim) : -1;
   // What the two kinds of parts take, roughly, in us on the whole chip: the bytes of their keys
@@ -923,6 +1046,16 @@ static int pa_with_form(int form, F&& f) {
 
 template <int DT, int D>
 static int pa_launch(const PrefixAttnParams& P, const PrefixPlan& pl, hipStream_t s) {
+  if (pl.whole) {
+    const unsigned grid = (unsigned)(P.B * P.Hkv);
+    constexpr int NW = PA_WHOLE_WAVES, lds = NW * 2 * PaGeo<D>::FEW_TILE;
+    static_assert(NW * 16 * (D * 4 + 8) + 64 <= lds, "the join of the waves fits their buffers");
+    KernelTimer timer("prefix_whole", s);
+    if (P.n * P.G <= 16) prefix_whole_kernel<DT, D, 1><<<grid, NW * 64, lds, s>>>(P);
+    else prefix_whole_kernel<DT, D, 2><<<grid, NW * 64, lds, s>>>(P);
+    timer.stop();
+    return check_launch("prefix_whole_kernel");
+  }
   // One launch for both kinds (a cache's columns are some of the prefix's: FS <= FP).
   const int64_t items = pl.items_p + pl.items_s;
   if (pl.form_p >= 0 && pl.form_s >= 0) {

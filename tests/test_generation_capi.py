@@ -118,14 +118,14 @@ def test_prefix_attention_refuses(kw, needle):
 
 
 def test_prefix_attention_wants_its_workspace():
-    a = attn()
+    a = attn(prefix_len=4096)
     lib = nat.lib()
     need = lib.nsmoe_prefix_attention_workspace_size(a)
     assert need > 0
     assert lib.nsmoe_prefix_attention(a, 256, need - 1, None) == 3
     assert lib.nsmoe_prefix_attention(a, None, need, None) == 3
     assert lib.nsmoe_prefix_attention(a, 264, need, None) == 1
-    with_weights = attn(weights_out=16)
+    with_weights = attn(prefix_len=4096, weights_out=16)
     assert lib.nsmoe_prefix_attention_workspace_size(with_weights) > need
 
 

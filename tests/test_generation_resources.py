@@ -10,7 +10,8 @@ import pytest
 from tests.test_kernel_resources import _of, kernels  # noqa: F401  (the fixture)
 
 
-@pytest.mark.parametrize("pattern", [r"prefix_part_kernel", r"prefix_join_kernel", r"rope_kernel",
+@pytest.mark.parametrize("pattern", [r"prefix_part_kernel", r"prefix_join_kernel",
+                                     r"prefix_whole_kernel", r"rope_kernel",
                                      r"evict_(select|move)_kernel", r"logits_kernel"])
 def test_nothing_is_spilled(kernels, pattern):  # noqa: F811
     for name, k in _of(kernels, pattern).items():

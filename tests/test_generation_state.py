@@ -1,13 +1,14 @@
 """
 What the generation operators keep track of, on the CPU: a decode cache whose step raised part
-way, its count of rows, and which heads a rotation's backward turns.
+way, its count of rows, which heads a rotation's backward turns, and which attentions are split
+into parts.
 """
 
 import pytest
 import torch
 
 pytest.importorskip("nanospeaker_amd.moe_kernel")
-from nanospeaker_amd import rope  # noqa: E402
+from nanospeaker_amd import _native as nat, rope  # noqa: E402
 from nanospeaker_amd.cache import DecodeCache  # noqa: E402
 
 
@@ -71,3 +72,18 @@ def test_backward_turns_the_heads_that_want_it(monkeypatch, need):
         assert (t.grad is not None) == want
         if want:
             assert torch.equal(t.grad, torch.full_like(t, 2))
+
+
+@pytest.mark.parametrize("kw,split", [
+    (dict(), False), (dict(prefix_len=0), False), (dict(prefix_len=1520), False),
+    (dict(prefix_len=1521), True), (dict(head_dim=128, prefix_len=752), False),
+    (dict(head_dim=128, prefix_len=753), True), (dict(prefix_len=4096, window=1024), False),
+    (dict(prefix_len=4096, window=1536, n_new=2), True), (dict(weights_out=16), True),
+    (dict(n_new=10), False), (dict(n_new=11), True), (dict(batch=400), True), (dict(cap=0), True)])
+def test_short_contexts_need_no_workspace(kw, split):
+    """One launch, without parts, for up to 32 columns a head over a short context."""
+    base = dict(dtype=0, head_dim=64, n_heads=9, n_kv_heads=3, batch=2, n_new=1, prefix_len=8,
+                cap=16, window=0, scale=0.125)
+    lib = nat.lib()
+    size = lib.nsmoe_prefix_attention_workspace_size(nat.PrefixAttnArgs(**(base | kw)))
+    assert (size > 0) == split

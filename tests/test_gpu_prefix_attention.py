@@ -152,6 +152,26 @@ def test_against_64_bits(dtype, b, n, p, s, hq, hk, d, window):
     run(case, window, weights=w)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("b,n,p,s,hq,hk,d,window", CASES)
+def test_without_weights_against_64_bits(dtype, b, n, p, s, hq, hk, d, window):
+    """Short contexts are not split where nobody asks for weights."""
+    print(f"[prefix] {dtype} {(b, n, p, s, hq, hk, d, window)}", flush=True)
+    run(make(b, n, p, s, hq, hk, d, dtype, seed=p + s + 1), window)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("n,g", [(1, 1), (5, 3), (16, 2)])
+@pytest.mark.parametrize("p,s", [(0, 40), (1, 33), (31, 64), (32, 31), (33, 1), (95, 97), (500, 520)])
+def test_short_contexts(d, n, g, p, s):
+    """Tiles that end with the prefix, with the window and with the sequence, in fewer tiles than
+    waves and in more."""
+    print(f"[prefix] short {(d, n, g, p, s)}", flush=True)
+    case = make(3, n, p, s, 2 * g, 2, d, torch.bfloat16, lens=[s, max(1, s // 2), min(s, n // 2)])
+    for window in (None, 1, 30, 70, p + 5):
+        run(case, window)
+
+
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("b", [1, 2, 4, 9])
 @pytest.mark.parametrize("n,g", [(5, 2), (5, 4), (10, 5), (20, 5), (25, 9)])
