@@ -48,8 +48,7 @@ int32_t nsmoe_abi_version(void);
  * main kernels ("pack", "route_fwd", "dispatch", "expert_fwd", "combine",
  * "expert_bwd", "expert_dx", "dw" (or "dw_in" and "dw_out" where they run apart),
  * "combine_dx", "router_dw", "route_bwd", "norm_bwd", "attn_k_prep", "attn_fwd", "ce_rows", "norm_fwd", "rope",
- * "logits", "evict_select", "evict_move",
- * "prefix_part", "prefix_join") until
+ * "logits", "evict_select", "evict_move", "prefix_part", "prefix_join", "prefix_whole") until
  * `capacity` pairs are used.
  * nsmoe_timing_read waits for the recorded events of one kernel and returns their
  * summed duration.  capacity 0 disables timing and frees the events. */
@@ -582,7 +581,8 @@ int nsmoe_cache_evict(const nsmoe_evict_args* args, void* stream);
  *     and the heads of its group; n_new * n_heads / n_kv_heads at most 64 with it.
  * 16-bit types, head_dim 64 or 128, scale > 0; pointers and strides multiples of 16 bytes, the
  * last dim contiguous.  Query head h reads key/value head h / (n_heads / n_kv_heads).
- * workspace: 16-byte aligned, nsmoe_prefix_attention_workspace_size(args) bytes. */
+ * workspace: 16-byte aligned, nsmoe_prefix_attention_workspace_size(args) bytes (0 for short
+ * contexts; it may be NULL then). */
 typedef struct nsmoe_prefix_attn_args {
   int32_t dtype;
   int32_t head_dim;

@@ -185,16 +185,20 @@ def test_every_pair_of_forms(d, b, n, g):
 
 
 @pytest.mark.parametrize("n,g", [(1, 3), (4, 3), (12, 4), (40, 5)])
-def test_rows_that_no_query_sees_may_hold_anything(n, g):
+@pytest.mark.parametrize("weights", [False, True])  # which keep the call in parts
+def test_rows_that_no_query_sees_may_hold_anything(n, g, weights):
     """NaN in every prefix and cache row before the oldest query's window."""
     q, kp, vp, k, v, lens = make(3, n, 100, 90, g, 1, 64, torch.bfloat16, lens=[90, 77, 50])
     k, v = clean(k), clean(v)
-    want = shared_prefix_attention(q, kp, vp, k, v, lens, window=8, return_lse=True)
+    kw = dict(window=8, return_lse=True)
+    if weights and n * g <= 64:
+        kw["weights_out"] = torch.empty(3, 1, 90, device=DEV)
+    want = shared_prefix_attention(q, kp, vp, k, v, lens, **kw)
     for i, ln in enumerate((90, 77, 50)):
         oldest = max(0, ln - n - 7)
         k[i, :oldest], v[i, :oldest] = NAN, NAN
     kp[:], vp[:] = NAN, NAN
-    got = shared_prefix_attention(q, kp, vp, k, v, lens, window=8, return_lse=True)
+    got = shared_prefix_attention(q, kp, vp, k, v, lens, **kw)
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
 
 
@@ -247,11 +251,12 @@ def test_scores_that_grow_along_the_keys():
     run((q, ramp(kp, 0).half(), vp, ramp(k, 1).half(), v, lens))
 
 
-def test_strided_operands():
+@pytest.mark.parametrize("p", [90, 1700])  # in one launch, in parts
+def test_strided_operands(p):
     """Keys and values as column blocks of a fused projection, heads before rows, a strided q."""
-    q, kp, vp, k, v, lens = make(3, 2, 90, 70, 9, 3, 64, torch.bfloat16)
+    q, kp, vp, k, v, lens = make(3, 2, p, 70, 9, 3, 64, torch.bfloat16)
     want = shared_prefix_attention(q, kp, vp, k, v, lens, return_lse=True)
-    fused = torch.full((90, 15, 64), NAN, dtype=q.dtype, device=DEV)
+    fused = torch.full((p, 15, 64), NAN, dtype=q.dtype, device=DEV)
     fused[:, 9:12], fused[:, 12:] = kp, vp
     caches = torch.full((3, 70, 15, 64), NAN, dtype=q.dtype, device=DEV)
     caches[:, :, 9:12], caches[:, :, 12:] = k, v
@@ -306,9 +311,10 @@ def test_offsets_past_32_bits():
     check(small, tail, q.dtype)
 
 
-def test_another_stream_and_two_calls_at_once():
-    a = make(4, 1, 300, 200, 9, 3, 64, torch.bfloat16, seed=1)
-    b = make(4, 1, 300, 200, 9, 3, 64, torch.bfloat16, seed=2)
+@pytest.mark.parametrize("p", [300, 1700])  # in one launch, in parts
+def test_another_stream_and_two_calls_at_once(p):
+    a = make(4, 1, p, 200, 9, 3, 64, torch.bfloat16, seed=1)
+    b = make(4, 1, p, 200, 9, 3, 64, torch.bfloat16, seed=2)
     want = [shared_prefix_attention(*c) for c in (a, b)]
     torch.cuda.synchronize()
     s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
@@ -347,8 +353,28 @@ def test_two_captured_graphs_replay_with_new_inputs():
                 assert torch.equal(x, y), seed
 
 
-def test_same_inputs_same_bits():
-    case = make(9, 2, 800, 300, 9, 3, 64, torch.bfloat16)
+@pytest.mark.parametrize("p", [300, 1700])  # in one launch, in parts
+def test_captured_without_weights(p):
+    held = make(4, 1, p, 200, 9, 3, 64, torch.bfloat16)
+    shared_prefix_attention(*held, return_lse=True)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        outs = shared_prefix_attention(*held, return_lse=True)
+    for seed in range(3):
+        new = make(4, 1, p, 200, 9, 3, 64, torch.bfloat16, seed=seed + 3)
+        for x, y in zip(held, new):
+            x.copy_(y)
+        g.replay()
+        got = [t.clone() for t in outs]
+        want = shared_prefix_attention(*new, return_lse=True)
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), seed
+
+
+@pytest.mark.parametrize("p", [800, 1700])  # in one launch, in parts
+def test_same_inputs_same_bits(p):
+    case = make(9, 2, p, 300, 9, 3, 64, torch.bfloat16)
     first = shared_prefix_attention(*case, return_lse=True)
     for _ in range(4):
         again = shared_prefix_attention(*case, return_lse=True)
