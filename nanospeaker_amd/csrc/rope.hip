@@ -16,8 +16,8 @@
 // and sines once, into LDS (they are shared by every head of the token), then stream the
 // heads of q and k, VP planes a thread and step in 16-byte vectors.  Bound by HBM at long calls
 // (each element read once and written once: 4 x 8192 tokens of 9 + 3 heads of 64, bf16, 17.8 us
-// or 5.6 TB/s out of a warm memory-side cache; 4 x 2047 of 32 + 8 heads of 128, fp32, 67 us, 5.0 TB/s)
-// and by launch latency at decode ones (64 tokens: 3.3 us).
+// or 5.6 TB/s out of a warm memory-side cache; 4 x 2047 of 32 + 8 heads of 128, fp32, 67 us or
+// 5.0 TB/s) and by launch latency at decode ones (64 tokens: 3.3 us).
 #include "../../include/nsmoe.h"
 #include "gemm_core.h"
 #include "nsmoe_capi_internal.h"

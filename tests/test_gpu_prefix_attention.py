@@ -213,6 +213,15 @@ def test_queries_without_a_row_and_lengths_out_of_range(lens, n, window):
         assert (got[2][i, :, max(0, min(ln, 40)):] == 1).all()  # rows behind keep theirs
 
 
+@pytest.mark.parametrize("lens", [[0, 0, 0], [1, 2, 3], [-7, 41, 2 ** 31 - 1]])
+@pytest.mark.parametrize("n", [1, 4])
+@pytest.mark.parametrize("p", [50, 1700])  # in one launch, in parts
+def test_lengths_out_of_range_without_weights(lens, n, p):
+    case = make(3, n, p, 40, 6, 2, 64, torch.bfloat16, lens=lens)
+    run(case)
+    run(case, window=3)
+
+
 def test_prefix_of_zero_rows_and_cache_of_zero_rows():
     q, kp, vp, k, v, lens = make(2, 1, 0, 9, 6, 2, 64, torch.bfloat16)
     a = run((q, kp, vp, k, v, lens))
